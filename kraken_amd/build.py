@@ -23,8 +23,10 @@ VARIANTS = {}
 HEADERS = [os.path.join(CSRC, 'common.h'),
            os.path.join(os.path.dirname(HERE), 'include', 'kraken_amd.h')]
 ARCH = 'gfx950'
+# packed-fp32-ops off: the compiler forms v_pk_{add,mul,fma}_f32 from ordinary float code by itself, and some of their forms have given
+# wrong results on this hardware now and then (the host pass warns that it does not know the feature: harmless)
 FLAGS = ['-O3', '-std=c++17', '-fPIC', f'--offload-arch={ARCH}', '-Wall', '-Wno-unused-function',
-         '-fno-gpu-rdc', '-DNDEBUG']
+         '-fno-gpu-rdc', '-DNDEBUG', '-Xclang', '-target-feature', '-Xclang', '-packed-fp32-ops']
 
 
 def _hipcc():
