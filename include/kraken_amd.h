@@ -50,7 +50,7 @@
 extern "C" {
 #endif
 
-#define KRK_ABI_VERSION 3   /* 3 (round 6): + krk_plan_clone; 2 (round 6): + krk_plan_get_recurrence; round 5 had added CONVT / RESHAPE ops, krk_plan_out_dims, krk_plan_olens_w, krk_plan_set_recurrence under version 1 */
+#define KRK_ABI_VERSION 4   /* 4: + the sequence operators and krk_constrain_logits; 3 (round 6): + krk_plan_clone; 2 (round 6): + krk_plan_get_recurrence; round 5 had added CONVT / RESHAPE ops, krk_plan_out_dims, krk_plan_olens_w, krk_plan_set_recurrence under version 1 */
 
 /* error codes */
 #define KRK_OK            0
@@ -318,6 +318,95 @@ int krk_dewarp_apply_page(const unsigned char* page_dev, long row_stride, int pi
  * sigmoid; one pass, (C, H, W) float32 out.
  */
 int krk_upsample_sigmoid(const float* x_dev, int C, int h, int w, int H, int W, float* y_dev, void* stream);
+
+/* ------------------------------------------------------------------------------------------------------------------------------
+ * Operators on sequence rows that are not part of a plan (no reference analogue: kraken's only mixer over a line's time axis is the
+ * LSTM, kraken/lib/vgsl/layers.py:462-547).  Rows are time-major, (n, t, channel) with adjacent channels; the other strides are the
+ * caller's, in ELEMENTS.  Ragged batches as everywhere here: only the first lens[n] steps of row n are valid (a DEVICE array, values
+ * are clamped to [0, T]; NULL: all T), steps behind them are neither read nor left undefined: outputs there are zero.
+ * Everything is enqueued on `stream`; nothing synchronises, allocates or keeps anything between calls, so the calls may be captured
+ * into a graph.  Sums, softmax statistics and states are fp32; 16-bit results are rounded once, at the end.  Buffers that a call
+ * writes must not overlap anything else it is given, except where said.
+ */
+#define KRK_TYPE_F32  0
+#define KRK_TYPE_BF16 1
+#define KRK_TYPE_F16  2
+
+/*
+ * Short depthwise causal convolution:  p_i = bias + sum_k weight[d][k] x[i - (K-1) + k][d],  y = p, or p * sigmoid(p) with `silu`.
+ * i counts the valid steps in processing order (reverse != 0: from the last one back), x in front of i = 0 comes from `state` (its
+ * row r is step r - (K-1)), or is zero.  state_out (may be NULL) receives the last K-1 inputs in the same form.
+ * With T == 1 state_out may be state itself: one step of a stream, in place.   1 <= K <= 8.
+ */
+typedef struct krk_conv_args {
+    const void* x; const void* weight; const void* bias; const void* state;   /* weight (D, K), bias (D) or NULL, of x's type */
+    void* y; void* state_out;
+    const int* lens;
+    long x_n, x_t, y_n, y_t, state_n, state_k, out_n, out_k;
+    int N, T, D, K, type, silu, reverse;
+} krk_conv_args;
+int krk_causal_conv(const krk_conv_args* args, void* stream);
+
+/*
+ * Selective state space scan, per channel d of group g = d / (D / G) with S states:
+ *     s_i = dt_i + dt_bias (softplus of it with `softplus`),  h_i = exp(s_i A) h_{i-1} + s_i x_i B_i,  y_i = C_i . h_i + skip x_i,
+ *     times z_i sigmoid(z_i) when z is given.
+ * Processing order, lens and padding as above.  A (D, S), skip (D), dt_bias (D) and the states (N, D, S) are fp32; skip, dt_bias, z,
+ * state (zero) and state_out may be NULL.  B, C (N, T, G, S): (G, S) adjacent.  With T == 1 state_out may be state itself.
+ * 1 <= S <= 256.  krk_selective_scan_workspace: bytes of device scratch that the call needs for these sizes (0: none; negative: error).
+ */
+typedef struct krk_scan_args {
+    const void* x; const void* dt; const void* B; const void* C; const void* z;
+    const float* A; const float* skip; const float* dt_bias; const float* state;
+    void* y; float* state_out;
+    const int* lens;
+    void* workspace; long workspace_bytes;
+    long x_n, x_t, dt_n, dt_t, b_n, b_t, c_n, c_t, z_n, z_t, y_n, y_t, state_n, out_n;
+    int N, T, D, S, G, type, softplus, reverse;
+} krk_scan_args;
+long krk_selective_scan_workspace(const krk_scan_args* args);
+int krk_selective_scan(const krk_scan_args* args, void* stream);
+
+/*
+ * Attention of Tq queries over Tk keys, H query heads sharing Hk key heads (head h reads key head h / (H / Hk)):
+ *     s = scale q.k;  cap > 0: s = cap tanh(s / cap);  slopes: s -= slopes[h] |p_i - j|;  softmax over the keys j that are allowed.
+ * p_i = i, or with align_end k_len - q_len + i (the last valid query stands at the last valid key).  Key j is allowed for query i if
+ * j < k_len, and documents[n][i] == documents[n][j] (Tq == Tk only), and, with causal, j <= p_i or j < prefix[n].
+ * A query without an allowed key, and every query i >= q_len, gives zeros.  Keys and values at j >= k_len are never used, whatever
+ * they hold; inside k_len a value that is not finite reaches only the queries that may see it.
+ * q, out (N, Tq, H, E), k, v (N, Tk, Hk, E): E adjacent.  1 <= E <= 256.  krk_attention_workspace as for the scan.
+ */
+typedef struct krk_attention_args {
+    const void* q; const void* k; const void* v; void* out;
+    const int* q_lens; const int* k_lens; const int* prefix; const int* documents;
+    const float* slopes;
+    void* workspace; long workspace_bytes;
+    long q_n, q_t, q_h, k_n, k_t, k_h, v_n, v_t, v_h, o_n, o_t, o_h, doc_n;
+    int N, Tq, Tk, H, Hk, E, type, causal, align_end;
+    float scale, cap;
+} krk_attention_args;
+long krk_attention_workspace(const krk_attention_args* args);
+int krk_attention(const krk_attention_args* args, void* stream);
+
+/*
+ * Constraint of scores in front of a decoder: for class c of row (n, t), with count = how often c occurs in history[n][0..hist_len),
+ *     count > 0: v = v > 0 ? v / repetition[n] : v * repetition[n];  v -= frequency[n] * count;  v -= presence[n];
+ *     v += bias[c];   -inf where bit c % 32 of mask word c / 32 is 0 (whatever the score holds).
+ * Every operation is rounded to fp32 on its own, the result once more to the scores' type.  logits, out (N, T, C): C adjacent; out may
+ * be logits.  history (N, L) int32 (hist64 == 0) or int64, labels outside [0, C) are ignored; hist_lens, bias, mask, history may be NULL;
+ * repetition / frequency / presence: fp32 (N) arrays, or NULL for the `all_` values; they have no effect without a history.
+ * bias_n: 0 = one row for all; mask_n, mask_t in words.
+ */
+typedef struct krk_constrain_args {
+    const void* logits; void* out;
+    const unsigned* mask; const float* bias;
+    const void* history; const int* hist_lens;
+    const float* repetition; const float* presence; const float* frequency;
+    long l_n, l_t, o_n, o_t, mask_n, mask_t, bias_n, hist_n;
+    int N, T, C, L, type, hist64;
+    float all_repetition, all_presence, all_frequency;
+} krk_constrain_args;
+int krk_constrain_logits(const krk_constrain_args* args, void* stream);
 
 /* Bytes of device workspace currently held by the plan (diagnostics). */
 long krk_plan_workspace_bytes(const krk_plan* plan);

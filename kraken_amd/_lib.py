@@ -29,7 +29,9 @@ EXPORTS = ['krk_abi_version', 'krk_last_error', 'krk_device_count', 'krk_plan_cr
            'krk_plan_layer_flops', 'krk_plan_num_steps', 'krk_plan_front_event', 'krk_plan_wait_front',
            'krk_plan_status', 'krk_prep_lines', 'krk_prep_crops', 'krk_upsample_sigmoid', 'krk_dewarp_measure', 'krk_dewarp_apply',
            'krk_prep_lines_fmt', 'krk_dewarp_measure_page', 'krk_dewarp_apply_page', 'krk_plan_has_exchange',
-           'krk_plan_set_recurrence', 'krk_plan_out_dims', 'krk_plan_olens_w', 'krk_plan_get_recurrence', 'krk_plan_clone']
+           'krk_plan_set_recurrence', 'krk_plan_out_dims', 'krk_plan_olens_w', 'krk_plan_get_recurrence', 'krk_plan_clone',
+           'krk_causal_conv', 'krk_selective_scan_workspace', 'krk_selective_scan', 'krk_attention_workspace', 'krk_attention',
+           'krk_constrain_logits']
 
 
 class KrkLayer(C.Structure):
@@ -42,6 +44,39 @@ class KrkLayer(C.Structure):
 class KrkDecodeOut(C.Structure):
     _fields_ = [('labels', C.c_void_p), ('starts', C.c_void_p), ('ends', C.c_void_p), ('confs', C.c_void_p),
                 ('counts', C.c_void_p), ('t_stride', C.c_int)]
+
+
+TYPE_F32, TYPE_BF16, TYPE_F16 = 0, 1, 2
+
+
+def _fields(pointers, longs, ints, floats=(), workspace=False):
+    f = [(n, C.c_void_p) for n in pointers]
+    if workspace:
+        f += [('workspace', C.c_void_p), ('workspace_bytes', C.c_long)]
+    return f + [(n, C.c_long) for n in longs] + [(n, C.c_int) for n in ints] + [(n, C.c_float) for n in floats]
+
+
+class KrkConvArgs(C.Structure):
+    _fields_ = _fields(['x', 'weight', 'bias', 'state', 'y', 'state_out', 'lens'],
+                       ['x_n', 'x_t', 'y_n', 'y_t', 'state_n', 'state_k', 'out_n', 'out_k'], ['N', 'T', 'D', 'K', 'type', 'silu', 'reverse'])
+
+
+class KrkScanArgs(C.Structure):
+    _fields_ = _fields(['x', 'dt', 'B', 'C', 'z', 'A', 'skip', 'dt_bias', 'state', 'y', 'state_out', 'lens'],
+                       ['x_n', 'x_t', 'dt_n', 'dt_t', 'b_n', 'b_t', 'c_n', 'c_t', 'z_n', 'z_t', 'y_n', 'y_t', 'state_n', 'out_n'],
+                       ['N', 'T', 'D', 'S', 'G', 'type', 'softplus', 'reverse'], workspace=True)
+
+
+class KrkAttentionArgs(C.Structure):
+    _fields_ = _fields(['q', 'k', 'v', 'out', 'q_lens', 'k_lens', 'prefix', 'documents', 'slopes'],
+                       ['q_n', 'q_t', 'q_h', 'k_n', 'k_t', 'k_h', 'v_n', 'v_t', 'v_h', 'o_n', 'o_t', 'o_h', 'doc_n'],
+                       ['N', 'Tq', 'Tk', 'H', 'Hk', 'E', 'type', 'causal', 'align_end'], ['scale', 'cap'], workspace=True)
+
+
+class KrkConstrainArgs(C.Structure):
+    _fields_ = _fields(['logits', 'out', 'mask', 'bias', 'history', 'hist_lens', 'repetition', 'presence', 'frequency'],
+                       ['l_n', 'l_t', 'o_n', 'o_t', 'mask_n', 'mask_t', 'bias_n', 'hist_n'], ['N', 'T', 'C', 'L', 'type', 'hist64'],
+                       ['all_repetition', 'all_presence', 'all_frequency'])
 
 
 class KrakenAmdError(RuntimeError):
@@ -58,7 +93,7 @@ def is_exchange_timeout(e: Exception) -> bool:
 
 
 RECURRENCE_AUTO, RECURRENCE_STREAMING = 0, 1
-ABI_VERSION = 3          # include/kraken_amd.h: KRK_ABI_VERSION
+ABI_VERSION = 4          # include/kraken_amd.h: KRK_ABI_VERSION
 
 
 class streaming_recurrence:
@@ -193,6 +228,13 @@ def load():
         lib.krk_dewarp_measure_page.restype = i32
         lib.krk_dewarp_apply_page.argtypes = [vp, i64, i32, vp, i32, i32, vp, vp, i32, i32, i32, vp, vp, vp]
         lib.krk_dewarp_apply_page.restype = i32
+        for name, args in (('krk_causal_conv', KrkConvArgs), ('krk_selective_scan', KrkScanArgs), ('krk_attention', KrkAttentionArgs),
+                           ('krk_constrain_logits', KrkConstrainArgs)):
+            getattr(lib, name).argtypes = [C.POINTER(args), vp]
+            getattr(lib, name).restype = i32
+        for name, args in (('krk_selective_scan_workspace', KrkScanArgs), ('krk_attention_workspace', KrkAttentionArgs)):
+            getattr(lib, name).argtypes = [C.POINTER(args)]
+            getattr(lib, name).restype = lng
         _lib = lib
     return _lib
 

@@ -1,0 +1,247 @@
+// Attention over sequence rows (krk_attention): tanh-capped scores, distance bias, document / prefix / causal / length masks, shared key heads.
+//
+//   s_j = scale q.k_j;  s_j = cap tanh(s_j / cap);  s_j -= slope |p - j|;  out = sum_j 2^(s'_j - m) v_j / sum_j 2^(s'_j - m),  s' = s log2 e
+//
+// Rows kernel: one query position of R heads that share a key head.  LE lanes share a key (16 bytes of it each), so a wave reads 64 / LE keys
+// at once; every group of lanes keeps its own running maximum, sum and output and they are joined at the end.  Keys and values are read
+// once per R heads: with one query position per row that is the memory bound.  A long axis is split over workgroups and joined by a second
+// launch where there are few rows.
+#include "seq.h"
+
+namespace {
+
+constexpr float LOG2E = 1.4426950408889634f;
+
+// cap tanh(s / cap).  fp32: the odd series below 0.45 (the rest is under 2^-25 of it), where 1 - 2 / (1 + e^2x) would cancel; 16-bit results
+// need no more than the latter.
+template <class T> __device__ __forceinline__ float seq_cap(float s, float cap, float rcap) {
+    const float x = s * rcap, ax = fabsf(x);
+    const float e = __builtin_amdgcn_exp2f(-2.f * LOG2E * ax);
+    float big = (1.f - e) * __builtin_amdgcn_rcpf(1.f + e);
+    if constexpr (sizeof(T) == 4) {
+        const float q = x * x;
+        float p = 21844.f / 6081075.f;
+        p = __builtin_fmaf(p, q, -1382.f / 155925.f);
+        p = __builtin_fmaf(p, q, 62.f / 2835.f);
+        p = __builtin_fmaf(p, q, -17.f / 315.f);
+        p = __builtin_fmaf(p, q, 2.f / 15.f);
+        p = __builtin_fmaf(p, q, -1.f / 3.f);
+        p = __builtin_fmaf(p * q, ax, ax);
+        big = ax < 0.45f ? p : big;
+    }
+    return cap * __builtin_copysignf(big, x);
+}
+
+struct Row {               // what the masks say about one query
+    int klen, limit, p;    // keys [0, klen), of which j < limit or (not causal): limit = max(p + 1, prefix)
+};
+__device__ __forceinline__ Row query_row(const krk_attention_args& a, int n, int i) {
+    Row r;
+    const int qlen = seq_len(a.q_lens, n, a.Tq);
+    r.klen = seq_len(a.k_lens, n, a.Tk);
+    r.p = a.align_end ? r.klen - qlen + i : i;
+    r.limit = r.klen;
+    if (a.causal) r.limit = min(r.klen, max(r.p + 1, a.prefix ? a.prefix[n] : 0));
+    if (i >= qlen) r.limit = 0;
+    return r;
+}
+
+template <class T, int R, int LE>
+__global__ __launch_bounds__(256) void attn_rows_kernel(krk_attention_args a, int blocks_h, int splits, int span) {
+    constexpr int V = VecOf<T>::V, KPW = 64 / LE, UK = 4;
+    const int rep = a.H / a.Hk;
+    long item = blockIdx.x;
+    const int rb = item % blocks_h; item /= blocks_h;
+    const int hk = item % a.Hk; item /= a.Hk;
+    const int i = item % a.Tq, n = item / a.Tq;
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, grp = lane / LE, e0 = (lane % LE) * V;
+    const int nv = max(0, min(V, a.E - e0));
+    const int h0 = hk * rep + rb * R, nr = min(R, rep - rb * R);
+    const Row row = query_row(a, n, i);
+    const int* docs = a.documents ? a.documents + n * a.doc_n : nullptr;
+    const int doc = docs && row.limit > 0 ? docs[i] : 0;
+    const float rcap = a.cap > 0.f ? 1.f / a.cap : 0.f;
+    const float qscale = a.cap > 0.f ? a.scale : a.scale * LOG2E;
+
+    float q[R][V], slope[R], m[R], l[R], o[R][V];
+#pragma unroll
+    for (int r = 0; r < R; ++r) {
+        const int h = h0 + (r < nr ? r : 0);
+        load_vec<T, V>((const T*)a.q + n * a.q_n + i * a.q_t + h * a.q_h + e0, nv, q[r]);
+#pragma unroll
+        for (int v = 0; v < V; ++v) q[r][v] *= qscale, o[r][v] = 0.f;
+        slope[r] = a.slopes ? a.slopes[h] * LOG2E : 0.f;
+        m[r] = -INFINITY;
+        l[r] = 0.f;
+    }
+    const T* kp = (const T*)a.k + n * a.k_n + hk * a.k_h + e0;
+    const T* vp = (const T*)a.v + n * a.v_n + hk * a.v_h + e0;
+    const int j0 = blockIdx.y * span, j1 = min(j0 + span, row.limit);
+    for (int jb = j0 + wave * KPW * UK; jb < j1; jb += 4 * KPW * UK) {
+        bool in[UK];
+        float kv[UK][V], vv[UK][V], s[UK][R];
+#pragma unroll
+        for (int u = 0; u < UK; ++u) {
+            const int j = jb + u * KPW + grp;
+            in[u] = j < j1 && (!docs || docs[j] == doc);
+            load_vec<T, V>(kp + (long)(in[u] ? j : 0) * a.k_t, in[u] ? nv : 0, kv[u]);
+            load_vec<T, V>(vp + (long)(in[u] ? j : 0) * a.v_t, in[u] ? nv : 0, vv[u]);
+        }
+#pragma unroll
+        for (int u = 0; u < UK; ++u)
+#pragma unroll
+            for (int r = 0; r < R; ++r) {
+                float d = 0.f;
+#pragma unroll
+                for (int v = 0; v < V; ++v) d = __builtin_fmaf(q[r][v], kv[u][v], d);
+#pragma unroll
+                for (int x = 1; x < LE; x <<= 1) d += __shfl_xor(d, x);
+                if (a.cap > 0.f) d = seq_cap<T>(d, a.cap, rcap) * LOG2E;
+                if (a.slopes) d = __builtin_fmaf(-slope[r], fabsf((float)(row.p - (jb + u * KPW + grp))), d);
+                s[u][r] = in[u] ? d : -INFINITY;
+            }
+#pragma unroll
+        for (int r = 0; r < R; ++r) {
+            float top = m[r];
+#pragma unroll
+            for (int u = 0; u < UK; ++u) top = fmaxf(top, s[u][r]);
+            const float ref = top == -INFINITY ? 0.f : top;
+            const float f = __builtin_amdgcn_exp2f(m[r] - ref);
+            m[r] = top;
+            l[r] *= f;
+#pragma unroll
+            for (int v = 0; v < V; ++v) o[r][v] *= f;
+#pragma unroll
+            for (int u = 0; u < UK; ++u) {
+                const float p = __builtin_amdgcn_exp2f(s[u][r] - ref);
+                l[r] += p;
+#pragma unroll
+                for (int v = 0; v < V; ++v) o[r][v] = __builtin_fmaf(p, vv[u][v], o[r][v]);
+            }
+        }
+    }
+    // join the groups of a wave, then the four waves
+    __shared__ float wm[4][R], wl[4][R], wo[4][R][LE * V];
+#pragma unroll
+    for (int r = 0; r < R; ++r) {
+        float top = m[r];
+#pragma unroll
+        for (int x = LE; x < 64; x <<= 1) top = fmaxf(top, __shfl_xor(top, x));
+        const float f = __builtin_amdgcn_exp2f(m[r] - (top == -INFINITY ? 0.f : top));   // 0 for a group that saw nothing
+        float sum = l[r] * f;
+#pragma unroll
+        for (int x = LE; x < 64; x <<= 1) sum += __shfl_xor(sum, x);
+#pragma unroll
+        for (int v = 0; v < V; ++v) {
+            float t = o[r][v] * f;
+#pragma unroll
+            for (int x = LE; x < 64; x <<= 1) t += __shfl_xor(t, x);
+            if (grp == 0) wo[wave][r][e0 + v] = t;
+        }
+        if (lane == 0) wm[wave][r] = top, wl[wave][r] = sum;
+    }
+    __syncthreads();
+    const long rows = (long)a.N * a.Tq * a.H;
+    for (int x = threadIdx.x; x < nr * a.E; x += 256) {
+        const int r = x / a.E, e = x - r * a.E;
+        float top = -INFINITY, sum = 0.f, t = 0.f;
+#pragma unroll
+        for (int w = 0; w < 4; ++w) top = fmaxf(top, wm[w][r]);
+#pragma unroll
+        for (int w = 0; w < 4; ++w) {
+            const float f = __builtin_amdgcn_exp2f(wm[w][r] - (top == -INFINITY ? 0.f : top));
+            sum = __builtin_fmaf(wl[w][r], f, sum);
+            t = __builtin_fmaf(wo[w][r][e], f, t);
+        }
+        if (splits == 1) {
+            ((T*)a.out)[n * a.o_n + i * a.o_t + (h0 + r) * a.o_h + e] = from_f<T>(sum == 0.f ? 0.f : t / sum);
+        } else {
+            float* ws = (float*)a.workspace;
+            const long at = (((long)n * a.Tq + i) * a.H + h0 + r) * splits + blockIdx.y;
+            ws[at * a.E + e] = t;
+            if (e == 0) {
+                float* ml = ws + rows * splits * a.E;
+                ml[at * 2] = top;
+                ml[at * 2 + 1] = sum;
+            }
+        }
+    }
+}
+
+// joins the splits of one row: a wave per row, lanes along E
+template <class T>
+__global__ __launch_bounds__(256) void attn_join_kernel(krk_attention_args a, int splits, long rows) {
+    const long row = (long)blockIdx.x * 4 + (threadIdx.x >> 6);
+    if (row >= rows) return;
+    const float* ws = (const float*)a.workspace;
+    const float* ml = ws + rows * splits * a.E + row * splits * 2;
+    float top = -INFINITY, sum = 0.f;
+    for (int x = 0; x < splits; ++x) top = fmaxf(top, ml[2 * x]);
+    const float ref = top == -INFINITY ? 0.f : top;
+    for (int x = 0; x < splits; ++x) sum = __builtin_fmaf(ml[2 * x + 1], __builtin_amdgcn_exp2f(ml[2 * x] - ref), sum);
+    const int h = row % a.H;
+    const long it = row / a.H;
+    const int i = it % a.Tq;
+    const long n = it / a.Tq;
+    for (int e = threadIdx.x & 63; e < a.E; e += 64) {
+        float t = 0.f;
+        for (int x = 0; x < splits; ++x) t = __builtin_fmaf(ws[(row * splits + x) * a.E + e], __builtin_amdgcn_exp2f(ml[2 * x] - ref), t);
+        ((T*)a.out)[n * a.o_n + i * a.o_t + h * a.o_h + e] = from_f<T>(sum == 0.f ? 0.f : t / sum);
+    }
+}
+
+int row_block(const krk_attention_args& a) {
+    const int rep = a.H / a.Hk;
+    return rep >= 8 ? 8 : rep >= 4 ? 4 : rep >= 2 ? 2 : 1;
+}
+
+// workgroups along the key axis: enough for four per CU where there are few rows, 256 keys at least for each
+int split_count(const krk_attention_args& a) {
+    const int rep = a.H / a.Hk, R = row_block(a);
+    const long items = (long)a.N * a.Tq * a.Hk * ((rep + R - 1) / R);
+    if (items <= 0 || a.Tk <= 0) return 1;
+    long want = (1024 + items - 1) / items, most = (a.Tk + 255) / 256;
+    return (int)max(1L, min(min(want, most), 1024L));
+}
+
+template <class T, int R, int LE>
+int launch_rows(const krk_attention_args& a, hipStream_t s) {
+    const int rep = a.H / a.Hk, blocks_h = (rep + R - 1) / R, splits = split_count(a);
+    int span = (a.Tk + splits - 1) / splits;
+    const long items = (long)a.N * a.Tq * a.Hk * blocks_h, rows = (long)a.N * a.Tq * a.H;
+    if (items > 0x7fffff00L) return -4;
+    hipLaunchKernelGGL((attn_rows_kernel<T, R, LE>), dim3((unsigned)items, splits), dim3(256), 0, s, a, blocks_h, splits, span);
+    if (splits > 1) hipLaunchKernelGGL((attn_join_kernel<T>), dim3((unsigned)((rows + 3) / 4)), dim3(256), 0, s, a, splits, rows);
+    return hipGetLastError() == hipSuccess ? 0 : -1;
+}
+
+template <class T, int R>
+int by_lanes(const krk_attention_args& a, hipStream_t s) {
+    const int need = (a.E + VecOf<T>::V - 1) / VecOf<T>::V;
+    if (need <= 8) return launch_rows<T, R, 8>(a, s);
+    if (need <= 16) return launch_rows<T, R, 16>(a, s);
+    if (need <= 32) return launch_rows<T, R, 32>(a, s);
+    if constexpr (sizeof(T) == 4) return launch_rows<T, R, 64>(a, s);
+    return -4;
+}
+
+template <class T>
+int by_rows(const krk_attention_args& a, hipStream_t s) {
+    switch (row_block(a)) {
+        case 8: return by_lanes<T, 8>(a, s);
+        case 4: return by_lanes<T, 4>(a, s);
+        case 2: return by_lanes<T, 2>(a, s);
+        default: return by_lanes<T, 1>(a, s);
+    }
+}
+
+}  // namespace
+
+long krk_attn_workspace(const krk_attention_args& a) {
+    const int splits = split_count(a);
+    return splits == 1 ? 0 : (long)a.N * a.Tq * a.H * splits * (a.E + 2) * (long)sizeof(float);
+}
+
+int krk_launch_attention(const krk_attention_args& a, hipStream_t s) {
+    return a.type == KRK_TYPE_F32 ? by_rows<float>(a, s) : a.type == KRK_TYPE_BF16 ? by_rows<bf16_t>(a, s) : by_rows<f16_t>(a, s);
+}

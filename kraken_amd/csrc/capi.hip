@@ -5,7 +5,7 @@
 // schedule and repacks the state-dict tensors into MFMA fragment order.
 // krk_forward plays the role of MultiParamSequential.forward (layers.py:44-53).
 #include "common.h"
-#include "../../include/kraken_amd.h"
+#include "seq.h"
 
 #include <algorithm>
 #include <cmath>
@@ -2645,6 +2645,81 @@ int krk_upsample_sigmoid(const float* x_dev, int C, int h, int w, int H, int W, 
     if (krk_launch_upsample_sigmoid(x_dev, y_dev, C, h, w, H, W, (hipStream_t)stream))
         return fail(KRK_E_HIP, std::string("krk_upsample_sigmoid: launch failed: ") + hipGetErrorString(hipGetLastError()));
     return KRK_OK;
+}
+
+// ---- operators on sequence rows (conv_seq.hip, scan_seq.hip, attn_seq.hip, constrain.hip)
+static bool seq_type(int t) { return t == KRK_TYPE_F32 || t == KRK_TYPE_BF16 || t == KRK_TYPE_F16; }
+
+// the common end of an operator: its launcher's answer as an error code
+static int seq_done(const char* who, int rc) {
+    if (rc == -4) return fail(KRK_E_UNSUPPORTED, std::string(who) + ": more rows than one launch can address");
+    if (rc) return fail(KRK_E_HIP, std::string(who) + ": launch failed: " + hipGetErrorString(hipGetLastError()));
+    return KRK_OK;
+}
+
+int krk_causal_conv(const krk_conv_args* a, void* stream) {
+    if (!a || !a->x || !a->weight || !a->y || a->N < 0 || a->T < 0 || a->D <= 0 || !seq_type(a->type))
+        return fail(KRK_E_INVALID, "krk_causal_conv: bad argument");
+    if (a->K < 1 || a->K > 8) return fail(KRK_E_UNSUPPORTED, "krk_causal_conv: kernels of 1 to 8 steps");
+    if (a->state_out && a->state_out == a->state && a->T != 1) return fail(KRK_E_INVALID, "krk_causal_conv: in place for one step only");
+    if (krk_device_count() <= 0) return fail(KRK_E_HIP, "krk_causal_conv: no HIP device");
+    if (a->N == 0 || (a->T == 0 && !a->state_out)) return KRK_OK;
+    return seq_done("krk_causal_conv", krk_launch_causal_conv(*a, (hipStream_t)stream));
+}
+
+static int scan_args_ok(const krk_scan_args* a) {
+    if (!a || !a->x || !a->dt || !a->A || !a->B || !a->C || !a->y || a->N < 0 || a->T < 0 || a->D <= 0 || !seq_type(a->type))
+        return fail(KRK_E_INVALID, "krk_selective_scan: bad argument");
+    if (a->S < 1 || a->S > 256) return fail(KRK_E_UNSUPPORTED, "krk_selective_scan: 1 to 256 states");
+    if (a->G < 1 || a->D % a->G) return fail(KRK_E_INVALID, "krk_selective_scan: groups must divide the channels");
+    if (a->state_out && a->state_out == a->state && a->T != 1) return fail(KRK_E_INVALID, "krk_selective_scan: in place for one step only");
+    return KRK_OK;
+}
+
+long krk_selective_scan_workspace(const krk_scan_args* a) {
+    if (int rc = scan_args_ok(a)) return rc;
+    return krk_scan_workspace(*a);
+}
+
+int krk_selective_scan(const krk_scan_args* a, void* stream) {
+    if (int rc = scan_args_ok(a)) return rc;
+    if (krk_device_count() <= 0) return fail(KRK_E_HIP, "krk_selective_scan: no HIP device");
+    if (a->N == 0 || (a->T == 0 && !a->state_out)) return KRK_OK;
+    const long need = krk_scan_workspace(*a);
+    if (need > 0 && (!a->workspace || a->workspace_bytes < need)) return fail(KRK_E_INVALID, "krk_selective_scan: workspace too small");
+    return seq_done("krk_selective_scan", krk_launch_selective_scan(*a, (hipStream_t)stream));
+}
+
+static int attention_args_ok(const krk_attention_args* a) {
+    if (!a || !a->q || !a->k || !a->v || !a->out || a->N < 0 || a->Tq < 0 || a->Tk < 0 || a->H <= 0 || a->Hk <= 0 || !seq_type(a->type))
+        return fail(KRK_E_INVALID, "krk_attention: bad argument");
+    if (a->H % a->Hk) return fail(KRK_E_INVALID, "krk_attention: key heads must divide the query heads");
+    if (a->E < 1 || a->E > 256) return fail(KRK_E_UNSUPPORTED, "krk_attention: heads of 1 to 256 channels");
+    if (a->documents && a->Tq != a->Tk) return fail(KRK_E_INVALID, "krk_attention: documents need as many queries as keys");
+    if (!(a->cap >= 0.f)) return fail(KRK_E_INVALID, "krk_attention: cap must not be negative");
+    return KRK_OK;
+}
+
+long krk_attention_workspace(const krk_attention_args* a) {
+    if (int rc = attention_args_ok(a)) return rc;
+    return krk_attn_workspace(*a);
+}
+
+int krk_attention(const krk_attention_args* a, void* stream) {
+    if (int rc = attention_args_ok(a)) return rc;
+    if (krk_device_count() <= 0) return fail(KRK_E_HIP, "krk_attention: no HIP device");
+    if (a->N == 0 || a->Tq == 0) return KRK_OK;
+    const long need = krk_attn_workspace(*a);
+    if (need > 0 && (!a->workspace || a->workspace_bytes < need)) return fail(KRK_E_INVALID, "krk_attention: workspace too small");
+    return seq_done("krk_attention", krk_launch_attention(*a, (hipStream_t)stream));
+}
+
+int krk_constrain_logits(const krk_constrain_args* a, void* stream) {
+    if (!a || !a->logits || !a->out || a->N < 0 || a->T < 0 || a->C <= 0 || a->L < 0 || !seq_type(a->type))
+        return fail(KRK_E_INVALID, "krk_constrain_logits: bad argument");
+    if (krk_device_count() <= 0) return fail(KRK_E_HIP, "krk_constrain_logits: no HIP device");
+    if (a->N == 0 || a->T == 0) return KRK_OK;
+    return seq_done("krk_constrain_logits", krk_launch_constrain(*a, (hipStream_t)stream));
 }
 
 // forward declaration: the v / 255 table shared by the preprocessing entry points
