@@ -15,12 +15,12 @@ HERE = os.path.dirname(os.path.abspath(__file__))
 CSRC = os.path.join(HERE, 'csrc')
 BUILD = os.path.join(CSRC, '_build')
 LIB = os.path.join(HERE, 'libkraken_amd.so')
-SOURCES = ['conv_mfma.hip', 'conv_x3.hip', 'conv_x3p.hip', 'conv_x6.hip', 'conv1_x3.hip', 'conv_taps_x3.hip', 'gemm_x3.hip', 'norm_x3.hip', 'lstm_rec.hip', 'lstm_small.hip', 'lstm_x3.hip', 'lstm_ws.hip', 'misc_kernels.hip', 'c1gn.hip', 'prep_lines.hip', 'dewarp.hip', 'conv_seq.hip', 'scan_seq.hip', 'attn_seq.hip', 'constrain.hip', 'capi.hip']
+SOURCES = ['conv_mfma.hip', 'conv_x3.hip', 'conv_x3p.hip', 'conv_x6.hip', 'conv1_x3.hip', 'conv_taps_x3.hip', 'gemm_x3.hip', 'norm_x3.hip', 'lstm_rec.hip', 'lstm_small.hip', 'lstm_x3.hip', 'lstm_ws.hip', 'misc_kernels.hip', 'c1gn.hip', 'prep_lines.hip', 'dewarp.hip', 'conv_seq.hip', 'scan_seq.hip', 'attn_seq.hip', 'attn_tile.hip', 'constrain.hip', 'capi.hip']
 # sources compiled a second time with -DKRK_BF16_ONE: the plain-bf16 plan's launchers (name_b1), see csrc/common.h
 ONE_TERM = ['conv1_x3.hip', 'conv_taps_x3.hip', 'conv_x3.hip', 'conv_x3p.hip', 'gemm_x3.hip', 'lstm_ws.hip']
 # further compiles of one source under a define (kernel experiments selected by a probe switch at run time): {source: [(suffix, -D...)]}
 VARIANTS = {}
-HEADERS = [os.path.join(CSRC, 'common.h'), os.path.join(CSRC, 'seq.h'),
+HEADERS = [os.path.join(CSRC, 'common.h'), os.path.join(CSRC, 'seq.h'), os.path.join(CSRC, 'attn_seq.h'),
            os.path.join(os.path.dirname(HERE), 'include', 'kraken_amd.h')]
 ARCH = 'gfx950'
 # packed-fp32-ops off: the compiler forms v_pk_{add,mul,fma}_f32 from ordinary float code by itself, and some of their forms have given

@@ -6,45 +6,9 @@
 // at once; every group of lanes keeps its own running maximum, sum and output and they are joined at the end.  Keys and values are read
 // once per R heads: with one query position per row that is the memory bound.  A long axis is split over workgroups and joined by a second
 // launch where there are few rows.
-#include "seq.h"
+#include "attn_seq.h"
 
 namespace {
-
-constexpr float LOG2E = 1.4426950408889634f;
-
-// cap tanh(s / cap).  fp32: the odd series below 0.45 (the rest is under 2^-25 of it), where 1 - 2 / (1 + e^2x) would cancel; 16-bit results
-// need no more than the latter.
-template <class T> __device__ __forceinline__ float seq_cap(float s, float cap, float rcap) {
-    const float x = s * rcap, ax = fabsf(x);
-    const float e = __builtin_amdgcn_exp2f(-2.f * LOG2E * ax);
-    float big = (1.f - e) * __builtin_amdgcn_rcpf(1.f + e);
-    if constexpr (sizeof(T) == 4) {
-        const float q = x * x;
-        float p = 21844.f / 6081075.f;
-        p = __builtin_fmaf(p, q, -1382.f / 155925.f);
-        p = __builtin_fmaf(p, q, 62.f / 2835.f);
-        p = __builtin_fmaf(p, q, -17.f / 315.f);
-        p = __builtin_fmaf(p, q, 2.f / 15.f);
-        p = __builtin_fmaf(p, q, -1.f / 3.f);
-        p = __builtin_fmaf(p * q, ax, ax);
-        big = ax < 0.45f ? p : big;
-    }
-    return cap * __builtin_copysignf(big, x);
-}
-
-struct Row {               // what the masks say about one query
-    int klen, limit, p;    // keys [0, klen), of which j < limit or (not causal): limit = max(p + 1, prefix)
-};
-__device__ __forceinline__ Row query_row(const krk_attention_args& a, int n, int i) {
-    Row r;
-    const int qlen = seq_len(a.q_lens, n, a.Tq);
-    r.klen = seq_len(a.k_lens, n, a.Tk);
-    r.p = a.align_end ? r.klen - qlen + i : i;
-    r.limit = r.klen;
-    if (a.causal) r.limit = min(r.klen, max(r.p + 1, a.prefix ? a.prefix[n] : 0));
-    if (i >= qlen) r.limit = 0;
-    return r;
-}
 
 template <class T, int R, int LE>
 __global__ __launch_bounds__(256) void attn_rows_kernel(krk_attention_args a, int blocks_h, int splits, int span) {
@@ -57,7 +21,7 @@ __global__ __launch_bounds__(256) void attn_rows_kernel(krk_attention_args a, in
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, grp = lane / LE, e0 = (lane % LE) * V;
     const int nv = max(0, min(V, a.E - e0));
     const int h0 = hk * rep + rb * R, nr = min(R, rep - rb * R);
-    const Row row = query_row(a, n, i);
+    const AttnRow row = query_row(a, n, i);
     const int* docs = a.documents ? a.documents + n * a.doc_n : nullptr;
     const int doc = docs && row.limit > 0 ? docs[i] : 0;
     const float rcap = a.cap > 0.f ? 1.f / a.cap : 0.f;
@@ -235,13 +199,35 @@ int by_rows(const krk_attention_args& a, hipStream_t s) {
     }
 }
 
+// One or two query positions read the keys as often as they are rows; more of them go to the tile kernel, which reads them once per block.
+bool by_tiles(const krk_attention_args& a) { return a.Tq > 2; }
+
+long part_bytes(const krk_attention_args& a, int splits) {
+    return splits == 1 ? 0 : ((long)a.N * a.Tq * a.H * splits * (a.E + 2) * (long)sizeof(float) + 15) / 16 * 16;
+}
+
+int launch_tiles(const krk_attention_args& a, hipStream_t s) {
+    const AttnTiles g = krk_attn_tiles(a);
+    const long rows = (long)a.N * a.Tq * a.H;
+    if (int rc = krk_launch_attn_tiles(a, g, (char*)a.workspace + part_bytes(a, g.splits), s)) return rc;
+    if (g.splits > 1) {
+        const dim3 grid((unsigned)((rows + 3) / 4));
+        if (a.type == KRK_TYPE_F32) hipLaunchKernelGGL((attn_join_kernel<float>), grid, dim3(256), 0, s, a, g.splits, rows);
+        else if (a.type == KRK_TYPE_BF16) hipLaunchKernelGGL((attn_join_kernel<bf16_t>), grid, dim3(256), 0, s, a, g.splits, rows);
+        else hipLaunchKernelGGL((attn_join_kernel<f16_t>), grid, dim3(256), 0, s, a, g.splits, rows);
+    }
+    return hipGetLastError() == hipSuccess ? 0 : -1;
+}
+
 }  // namespace
 
 long krk_attn_workspace(const krk_attention_args& a) {
-    const int splits = split_count(a);
-    return splits == 1 ? 0 : (long)a.N * a.Tq * a.H * splits * (a.E + 2) * (long)sizeof(float);
+    if (!by_tiles(a)) return part_bytes(a, split_count(a));
+    const AttnTiles g = krk_attn_tiles(a);
+    return part_bytes(a, g.splits) + g.range_bytes;
 }
 
 int krk_launch_attention(const krk_attention_args& a, hipStream_t s) {
+    if (by_tiles(a)) return launch_tiles(a, s);
     return a.type == KRK_TYPE_F32 ? by_rows<float>(a, s) : a.type == KRK_TYPE_BF16 ? by_rows<bf16_t>(a, s) : by_rows<f16_t>(a, s);
 }

@@ -1,0 +1,482 @@
+// Attention of many queries: a workgroup of NW waves holds NW * 32 queries of one head and walks the key tiles that its masks leave.
+//
+// Scores are computed transposed, S^T = K Q^T on 32x32 matrix instructions: a lane then owns ONE query (its column) and 16 keys per block, so
+// the running maximum and sum of the softmax are registers of a lane plus one exchange with the lane 32 away, and the weights are already the B
+// operand of the second product O^T = V^T P^T -- the order of the keys inside a contraction is free, so V is read in the order in which the
+// scores lie.  16-bit types: 32x32x16, V^T by transposing LDS reads (ds_read_b64_tr_b16) from row-major tiles.  fp32: the exact 32x32x2.
+// Key tiles pass through LDS, the next one's loads are in flight while a tile is computed.
+#include "attn_seq.h"
+
+namespace {
+
+typedef short s16x4 __attribute__((ext_vector_type(4)));
+typedef short s16x8 __attribute__((ext_vector_type(8)));
+typedef __bf16 bf16x8 __attribute__((ext_vector_type(8)));
+typedef _Float16 f16x8 __attribute__((ext_vector_type(8)));
+typedef unsigned u32x4 __attribute__((ext_vector_type(4)));
+
+__device__ __forceinline__ f32x16 mfma16(bf16_t, const s16x8& a, const s16x8& b, const f32x16& c) {
+    return __builtin_amdgcn_mfma_f32_32x32x16_bf16(__builtin_bit_cast(bf16x8, a), __builtin_bit_cast(bf16x8, b), c, 0, 0, 0);
+}
+__device__ __forceinline__ f32x16 mfma16(f16_t, const s16x8& a, const s16x8& b, const f32x16& c) {
+    return __builtin_amdgcn_mfma_f32_32x32x16_f16(__builtin_bit_cast(f16x8, a), __builtin_bit_cast(f16x8, b), c, 0, 0, 0);
+}
+__device__ __forceinline__ f32x16 mfma16(float, const s16x8&, const s16x8&, const f32x16& c) { return c; }
+
+// exponent bits all ones: infinity or NaN
+template <class T> __device__ __forceinline__ bool odd_value(unsigned short v) {
+    constexpr unsigned short M = sizeof(T) == 2 && __is_same(T, bf16_t) ? 0x7f80 : 0x7c00;
+    return (v & M) == M;
+}
+__device__ __forceinline__ bool odd_float(float v) { return (__builtin_bit_cast(unsigned, v) & 0x7f800000u) == 0x7f800000u; }
+
+// What an odd value does to a sum, as numbers a matrix product can count: 1 for NaN, 128 for +inf, 16384 for -inf; at most 64 keys of each in a
+// tile, so the counts stay apart and exact in fp32.
+__device__ __forceinline__ float odd_mark(float v) { return v != v ? 1.f : v > 0.f ? 128.f : 16384.f; }
+__device__ __forceinline__ float odd_sum(float count) {
+    const int c = (int)count, nan = c & 127, pos = (c >> 7) & 127, neg = c >> 14;
+    if (c == 0) return 0.f;
+    return nan || (pos && neg) ? __builtin_nanf("") : pos ? INFINITY : -INFINITY;
+}
+
+template <class T, int EP> struct Geo {
+    static constexpr bool F32 = sizeof(T) == 4;
+    static constexpr int BK = F32 ? 32 : 64;                              // keys of a tile
+    static constexpr int SB = BK / 32, EB = EP / 32;
+    static constexpr int KLD = F32 ? EP + 4 : EP + 8;                     // row pitches (elements) that spread a read over the banks:
+    static constexpr int VLD = F32 ? EP + 8 : EP + (EP % 128 ? (EP % 64 ? 0 : 32) : 32);   // K rows by 16 bytes, V rows by quads of rows
+    static constexpr int CV = VecOf<T>::V;                                // elements of a 16-byte chunk
+    static constexpr int CHUNKS = BK * EP / CV;
+};
+
+// tile key ranges of the documents: min and max id of every tile's valid keys
+__global__ __launch_bounds__(256) void attn_ranges_kernel(krk_attention_args a, int2* out, int tiles, int keys) {
+    const long id = (long)blockIdx.x * 4 + (threadIdx.x >> 6);
+    if (id >= (long)a.N * tiles) return;
+    const int n = id / tiles, t = id % tiles, lane = threadIdx.x & 63;
+    const int j = t * keys + lane;
+    const bool in = lane < keys && j < seq_len(a.k_lens, n, a.Tk);
+    int lo = in ? a.documents[n * a.doc_n + j] : 0x7fffffff, hi = in ? lo : (int)0x80000000;
+#pragma unroll
+    for (int x = 1; x < 64; x <<= 1) lo = min(lo, __shfl_xor(lo, x)), hi = max(hi, __shfl_xor(hi, x));
+    if (lane == 0) out[id] = make_int2(lo, hi);
+}
+
+template <class T, int EP, int NW>
+__global__ __launch_bounds__(NW * 64) void attn_tile_kernel(krk_attention_args a, int qblocks, int splits, int tiles, const int2* ranges) {
+    using G = Geo<T, EP>;
+    constexpr bool F32 = G::F32;
+    constexpr int BK = G::BK, SB = G::SB, EB = G::EB, KLD = G::KLD, VLD = G::VLD, CV = G::CV, NT = NW * 64;
+    constexpr int CPT = (G::CHUNKS + NT - 1) / NT, CPR = EP / CV;         // chunks per thread and per row
+    __shared__ __attribute__((aligned(16))) T Ks[BK * KLD];
+    __shared__ __attribute__((aligned(16))) T Vs[BK * VLD];
+    __shared__ int dks[BK];
+    __shared__ int odd[2];
+
+    // All query blocks and heads that share a key head run on one XCD (workgroups go round the eight of them), so its L2 holds their keys; the
+    // blocks with the longest causal rows first.
+    const int rep = a.H / a.Hk, inner = qblocks * rep;
+    const long id = blockIdx.x / 8;
+    const long kvh = (blockIdx.x & 7) + 8 * (id / inner);
+    if (kvh >= (long)a.N * a.Hk) return;
+    const int n = kvh / a.Hk, hk = kvh % a.Hk, in = id % inner;
+    const int h = hk * rep + in % rep, q0 = (qblocks - 1 - in / rep) * NW * 32;
+    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), half = lane >> 5, col = lane & 31;
+    const int qlen = seq_len(a.q_lens, n, a.Tq), split = blockIdx.y;
+    const int qi = q0 + wave * 32 + col;                                  // this lane's query
+    T* out = (T*)a.out + n * a.o_n + h * a.o_h;
+    const int* docs = a.documents ? a.documents + n * a.doc_n : nullptr;
+
+    // what the masks say: about this lane's query, about the wave's first (the shortest reach) and last one, about the workgroup
+    const AttnRow mine = query_row(a, n, min(qi, a.Tq - 1));
+    const int lim = qi < qlen ? mine.limit : 0;
+    const int wfirst = q0 + wave * 32, wlast = min(wfirst + 31, qlen - 1);
+    const bool awake = wfirst < qlen;
+    const int wmin = awake ? query_row(a, n, wfirst).limit : 0, wmax = awake ? query_row(a, n, wlast).limit : 0;
+    const int bfirst = min(q0, qlen - 1), blast = min(q0 + NW * 32, qlen) - 1;
+    const int bmax = q0 < qlen ? query_row(a, n, blast).limit : 0;
+    const int bmin = q0 < qlen ? query_row(a, n, bfirst).limit : 0;
+    int doc = 0, wlo = 0, whi = 0, blo = 0, bhi = 0;
+    if (docs && q0 < qlen) {
+        doc = docs[min(qi, qlen - 1)];
+        wlo = whi = doc;
+        blo = 0x7fffffff, bhi = (int)0x80000000;
+        for (int i = lane; i < NW * 32; i += 64) {
+            const int d = docs[min(q0 + i, qlen - 1)];
+            blo = min(blo, d), bhi = max(bhi, d);
+        }
+#pragma unroll
+        for (int x = 1; x < 64; x <<= 1) {
+            wlo = min(wlo, __shfl_xor(wlo, x)), whi = max(whi, __shfl_xor(whi, x));
+            blo = min(blo, __shfl_xor(blo, x)), bhi = max(bhi, __shfl_xor(bhi, x));
+        }
+    }
+
+    // the query as B operand: column = query.  16-bit: 8 channels from 16 ks + 8 half; fp32: 4 from 8 g + 4 half.  A negative scale turns its sign.
+    const float sign = a.scale > 0.f ? 1.f : a.scale < 0.f ? -1.f : 0.f;
+    const float c = (a.scale != 0.f ? fabsf(a.scale) : 1.f) * LOG2E;
+    s16x8 q16[F32 ? 1 : EP / 16];
+    f32x4 q32[F32 ? EP / 8 : 1];
+    {
+        const T* qp = (const T*)a.q + n * a.q_n + (long)min(qi, a.Tq - 1) * a.q_t + h * a.q_h;
+        if constexpr (F32) {
+#pragma unroll
+            for (int g = 0; g < EP / 8; ++g) {
+                float v[4];
+                load_vec<float, 4>(qp + 8 * g + 4 * half, a.E - 8 * g - 4 * half, v);
+#pragma unroll
+                for (int i = 0; i < 4; ++i) q32[g][i] = v[i] * sign;
+            }
+        } else {
+#pragma unroll
+            for (int ks = 0; ks < EP / 16; ++ks) {
+                float v[8];
+                load_vec<T, 8>(qp + 16 * ks + 8 * half, a.E - 16 * ks - 8 * half, v);
+#pragma unroll
+                for (int i = 0; i < 8; ++i) q16[ks][i] = __builtin_bit_cast(short, from_f<T>(v[i] * sign));
+            }
+        }
+    }
+    const float slope = a.slopes ? a.slopes[h] * LOG2E : 0.f;
+    const float rcap = a.cap > 0.f ? 1.f / a.cap : 0.f;
+    const bool plain = a.cap <= 0.f && !a.slopes;
+
+    f32x16 o[EB];
+#pragma unroll
+    for (int eb = 0; eb < EB; ++eb)
+#pragma unroll
+        for (int i = 0; i < 16; ++i) o[eb][i] = 0.f;
+    float m = -INFINITY, l = 0.f;
+
+    // the tiles of this split that the masks leave, 64 at a time as bits
+    const int want = (bmax + BK - 1) / BK;
+    const int span = (tiles + splits - 1) / splits;
+    const int t1 = min(want, (split + 1) * span);
+    int base = split * span - 64;
+    unsigned long long left = 0;
+    auto next = [&]() -> int {
+        while (!left) {
+            base += 64;
+            if (base >= t1) return -1;
+            const int t = base + lane;
+            bool in = t < t1;
+            if (docs && in) {
+                const int2 r = ranges[(long)n * tiles + t];
+                in = r.x <= bhi && r.y >= blo;
+            }
+            left = __ballot(in);
+        }
+        const int b = __builtin_ctzll(left);
+        left &= left - 1;
+        return base + b;
+    };
+
+    const T* kp = (const T*)a.k + n * a.k_n + hk * a.k_h;
+    const T* vp = (const T*)a.v + n * a.v_n + hk * a.v_h;
+    u32x4 kr[CPT], vr[CPT];
+    int dr = 0;
+    auto fetch = [&](int t) {
+#pragma unroll
+        for (int x = 0; x < CPT; ++x) {
+            const int id = threadIdx.x + x * NT, row = id / CPR, e = (id - row * CPR) * CV;
+            const int j = t * BK + row;
+            kr[x] = vr[x] = (u32x4){0, 0, 0, 0};
+            if ((G::CHUNKS % NT == 0 || id < G::CHUNKS) && j < mine.klen) {
+                const T *ks = kp + (long)j * a.k_t + e, *vs = vp + (long)j * a.v_t + e;
+                if (e + CV <= a.E) {
+                    __builtin_memcpy(&kr[x], ks, 16);
+                    __builtin_memcpy(&vr[x], vs, 16);
+                } else if (e < a.E) {
+                    T kt[CV] = {}, vt[CV] = {};
+#pragma unroll
+                    for (int i = 0; i < CV; ++i)
+                        if (e + i < a.E) kt[i] = ks[i], vt[i] = vs[i];
+                    __builtin_memcpy(&kr[x], kt, 16);
+                    __builtin_memcpy(&vr[x], vt, 16);
+                }
+            }
+        }
+        if (docs && threadIdx.x < BK) dr = docs[min(t * BK + (int)threadIdx.x, a.Tk - 1)];
+    };
+
+    if (threadIdx.x < 2) odd[threadIdx.x] = 0;
+    int tile = next(), turn = 0;
+    if (tile >= 0) fetch(tile);
+    while (tile >= 0) {
+        __syncthreads();                                                  // the tile before is used up
+        const int t = tile, k0 = t * BK;
+        // A value that is not finite must not reach the queries that may not see it: 0 x NaN is NaN.  Only tiles that some query of the workgroup
+        // sees in part can do that; they are searched while they go to LDS.
+        const bool search = k0 + BK > bmin || docs;
+        bool found = false;
+#pragma unroll
+        for (int x = 0; x < CPT; ++x) {
+            const int id = threadIdx.x + x * NT, row = id / CPR, e = (id - row * CPR) * CV;
+            if (G::CHUNKS % NT == 0 || id < G::CHUNKS) {
+                *(u32x4*)&Ks[row * KLD + e] = kr[x];
+                *(u32x4*)&Vs[row * VLD + e] = vr[x];
+                if (search) {
+#pragma unroll
+                    for (int i = 0; i < 4; ++i) {
+                        const unsigned w = vr[x][i];
+                        if constexpr (F32) found |= odd_float(__builtin_bit_cast(float, w));
+                        else found |= odd_value<T>(w & 0xffff) || odd_value<T>(w >> 16);
+                    }
+                }
+            }
+        }
+        if (found) odd[turn & 1] = 1;
+        if (docs && threadIdx.x < BK) dks[threadIdx.x] = dr;
+        __syncthreads();
+        const bool bad = search && odd[turn & 1];
+        if (threadIdx.x == 0) odd[(turn + 1) & 1] = 0;
+        ++turn;
+        tile = next();
+        if (tile >= 0) fetch(tile);
+
+        if (!awake || k0 >= wmax) continue;
+        bool part = k0 + BK > wmin;
+        if (docs) {
+            const int2 r = ranges[(long)n * tiles + t];
+            if (r.x > whi || r.y < wlo) continue;
+            part = part || r.x != r.y || wlo != whi;
+        }
+
+        // S^T = K Q^T
+        f32x16 s[SB];
+#pragma unroll
+        for (int b = 0; b < SB; ++b) {
+#pragma unroll
+            for (int i = 0; i < 16; ++i) s[b][i] = 0.f;
+            const T* kb = &Ks[(b * 32 + col) * KLD];
+            if constexpr (F32) {
+#pragma unroll
+                for (int g = 0; g < EP / 8; ++g) {
+                    const f32x4 k = *(const f32x4*)&kb[8 * g + 4 * half];
+#pragma unroll
+                    for (int i = 0; i < 4; ++i) s[b] = __builtin_amdgcn_mfma_f32_32x32x2f32(k[i], q32[g][i], s[b], 0, 0, 0);
+                }
+            } else {
+#pragma unroll
+                for (int ks = 0; ks < EP / 16; ++ks) s[b] = mfma16(T{}, *(const s16x8*)&kb[16 * ks + 8 * half], q16[ks], s[b]);
+            }
+        }
+        // register i of block b: key k0 + 32 b + 8 (i / 4) + 4 half + i % 4
+        float scale = c;
+        if (!plain) {
+            scale = 1.f;
+            const float d0 = (float)(mine.p - k0 - 4 * half);
+            if (a.cap > 0.f) {
+                if constexpr (F32) {
+                    const float raw = c * (1.f / LOG2E);
+#pragma unroll
+                    for (int b = 0; b < SB; ++b)
+#pragma unroll
+                        for (int i = 0; i < 16; ++i) s[b][i] = seq_cap<T>(s[b][i] * raw, a.cap, rcap) * LOG2E;
+                } else {                                                  // cap tanh(x) = cap - 2 cap / (1 + e^2x): 2^-23 of cap off at most
+                    const float cl = a.cap * LOG2E, cx = 2.f * c * rcap;
+#pragma unroll
+                    for (int b = 0; b < SB; ++b)
+#pragma unroll
+                        for (int i = 0; i < 16; ++i)
+                            s[b][i] = __builtin_fmaf(-2.f * cl, __builtin_amdgcn_rcpf(1.f + __builtin_amdgcn_exp2f(s[b][i] * cx)), cl);
+                }
+            } else {
+#pragma unroll
+                for (int b = 0; b < SB; ++b)
+#pragma unroll
+                    for (int i = 0; i < 16; ++i) s[b][i] *= c;
+            }
+            if (a.slopes)
+#pragma unroll
+                for (int b = 0; b < SB; ++b)
+#pragma unroll
+                    for (int i = 0; i < 16; ++i)
+                        s[b][i] = __builtin_fmaf(-slope, fabsf(d0 - (float)(32 * b + 8 * (i / 4) + i % 4)), s[b][i]);
+        }
+        if (part) {
+            const int room = lim - k0 - 4 * half;
+#pragma unroll
+            for (int b = 0; b < SB; ++b)
+#pragma unroll
+                for (int i = 0; i < 16; ++i) {
+                    const int x = 32 * b + 8 * (i / 4) + i % 4;
+                    bool ok = x < room;
+                    if (docs) ok = ok && dks[x + 4 * half] == doc;
+                    s[b][i] = ok ? s[b][i] : -INFINITY;
+                }
+        }
+        float top = s[0][0];
+#pragma unroll
+        for (int b = 0; b < SB; ++b)
+#pragma unroll
+            for (int i = 0; i < 16; ++i) top = fmaxf(top, s[b][i]);
+        top = fmaxf(top, __shfl_xor(top, 32)) * scale;
+        // The reference point moves only when a score passes it by 2^8: weights up to 256 are as exact, and most tiles leave the sums alone.
+        if (__ballot(top > m + 8.f)) {
+            const float nm = fmaxf(m, top), f = __builtin_amdgcn_exp2f(m - (nm == -INFINITY ? 0.f : nm));
+            m = nm;
+            l *= f;
+#pragma unroll
+            for (int eb = 0; eb < EB; ++eb)
+#pragma unroll
+                for (int i = 0; i < 16; ++i) o[eb][i] *= f;
+        }
+        const float ref = m == -INFINITY ? 0.f : m;
+        float sum = 0.f;
+#pragma unroll
+        for (int b = 0; b < SB; ++b)
+#pragma unroll
+            for (int i = 0; i < 16; ++i) {
+                s[b][i] = __builtin_amdgcn_exp2f(__builtin_fmaf(s[b][i], scale, -ref));
+                sum += s[b][i];
+            }
+        l += sum;
+
+        // O^T += V^T P^T
+        if constexpr (F32) {
+#pragma unroll
+            for (int eb = 0; eb < EB; ++eb) {
+                f32x16 marks;
+                if (bad)
+#pragma unroll
+                    for (int i = 0; i < 16; ++i) marks[i] = 0.f;
+#pragma unroll
+                for (int b = 0; b < SB; ++b)
+#pragma unroll
+                    for (int i = 0; i < 16; ++i) {
+                        float v = Vs[(b * 32 + 8 * (i / 4) + i % 4 + 4 * half) * VLD + eb * 32 + col];
+                        if (bad) {
+                            const bool is = odd_float(v);
+                            marks = __builtin_amdgcn_mfma_f32_32x32x2f32(is ? odd_mark(v) : 0.f, s[b][i] > 0.f ? 1.f : s[b][i], marks, 0, 0, 0);
+                            v = is ? 0.f : v;
+                        }
+                        o[eb] = __builtin_amdgcn_mfma_f32_32x32x2f32(v, s[b][i], o[eb], 0, 0, 0);
+                    }
+                if (bad)
+#pragma unroll
+                    for (int i = 0; i < 16; ++i) o[eb][i] += odd_sum(marks[i]);
+            }
+        } else {
+            s16x8 p[SB * 2];
+#pragma unroll
+            for (int x = 0; x < SB * 2; ++x)
+#pragma unroll
+                for (int i = 0; i < 8; ++i) p[x][i] = __builtin_bit_cast(short, from_f<T>(s[x / 2][8 * (x & 1) + i]));
+            const int vrow = 4 * half + (col & 15) / 4, vcol = 16 * (col >> 4) + 4 * (col & 3);
+#pragma unroll
+            for (int eb = 0; eb < EB; ++eb) {
+                s16x8 v[SB * 2];
+#pragma unroll
+                for (int x = 0; x < SB * 2; ++x) {
+                    typedef __attribute__((address_space(3))) s16x4 lds4;
+                    const s16x4 lo = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds4*)&Vs[(16 * x + vrow) * VLD + eb * 32 + vcol]);
+                    const s16x4 hi = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds4*)&Vs[(16 * x + 8 + vrow) * VLD + eb * 32 + vcol]);
+                    v[x] = __builtin_shufflevector(lo, hi, 0, 1, 2, 3, 4, 5, 6, 7);
+                }
+                if (bad) {
+                    f32x16 marks;
+#pragma unroll
+                    for (int i = 0; i < 16; ++i) marks[i] = 0.f;
+#pragma unroll
+                    for (int x = 0; x < SB * 2; ++x) {
+                        s16x8 mark, one;
+#pragma unroll
+                        for (int i = 0; i < 8; ++i) {
+                            const bool is = odd_value<T>((unsigned short)v[x][i]);
+                            mark[i] = __builtin_bit_cast(short, from_f<T>(is ? odd_mark(to_f(__builtin_bit_cast(T, v[x][i]))) : 0.f));
+                            const float w = s[x / 2][8 * (x & 1) + i];
+                            one[i] = __builtin_bit_cast(short, from_f<T>(w > 0.f ? 1.f : w));
+                            if (is) v[x][i] = 0;
+                        }
+                        marks = mfma16(T{}, mark, one, marks);
+                    }
+#pragma unroll
+                    for (int i = 0; i < 16; ++i) o[eb][i] += odd_sum(marks[i]);
+                }
+#pragma unroll
+                for (int x = 0; x < SB * 2; ++x) o[eb] = mfma16(T{}, v[x], p[x], o[eb]);
+            }
+        }
+    }
+
+    l += __shfl_xor(l, 32);
+    if (qi >= a.Tq) return;
+    if (splits == 1) {
+        const float r = lim > 0 && l != 0.f ? 1.f / l : 0.f;
+#pragma unroll
+        for (int eb = 0; eb < EB; ++eb)
+#pragma unroll
+            for (int g = 0; g < 4; ++g) {
+                const int e = eb * 32 + 8 * g + 4 * half;
+                float v[4];
+#pragma unroll
+                for (int i = 0; i < 4; ++i) v[i] = lim > 0 && l != 0.f ? o[eb][4 * g + i] * r : 0.f;
+                store_vec<T, 4>(out + (long)qi * a.o_t + e, a.E - e, v);
+            }
+    } else {
+        float* ws = (float*)((char*)a.workspace);
+        const long rows = (long)a.N * a.Tq * a.H, at = (((long)n * a.Tq + qi) * a.H + h) * splits + split;
+        const bool any = lim > 0;
+#pragma unroll
+        for (int eb = 0; eb < EB; ++eb)
+#pragma unroll
+            for (int g = 0; g < 4; ++g) {
+                const int e = eb * 32 + 8 * g + 4 * half;
+                float v[4];
+#pragma unroll
+                for (int i = 0; i < 4; ++i) v[i] = any ? o[eb][4 * g + i] : 0.f;
+                store_vec<float, 4>(ws + at * a.E + e, a.E - e, v);
+            }
+        if (half == 0) {
+            ws[rows * splits * a.E + at * 2] = any ? m : -INFINITY;
+            ws[rows * splits * a.E + at * 2 + 1] = any ? l : 0.f;
+        }
+    }
+}
+
+template <class T, int EP, int NW>
+int launch(const krk_attention_args& a, const AttnTiles& g, void* scratch, hipStream_t s) {
+    const int qblocks = (a.Tq + NW * 32 - 1) / (NW * 32), tiles = (a.Tk + g.keys - 1) / g.keys;
+    const int2* ranges = nullptr;
+    if (a.documents) {
+        int2* r = (int2*)scratch;
+        ranges = r;
+        hipLaunchKernelGGL(attn_ranges_kernel, dim3((unsigned)(((long)a.N * tiles + 3) / 4)), dim3(256), 0, s, a, r, tiles, g.keys);
+    }
+    const long blocks = ((long)a.N * a.Hk + 7) / 8 * 8 * qblocks * (a.H / a.Hk);
+    if (blocks > 0x7fffff00L) return -4;
+    hipLaunchKernelGGL((attn_tile_kernel<T, EP, NW>), dim3((unsigned)blocks, g.splits), dim3(NW * 64), 0, s, a, qblocks, g.splits, tiles, ranges);
+    return hipGetLastError() == hipSuccess ? 0 : -1;
+}
+
+template <class T, int EP>
+int by_waves(const krk_attention_args& a, const AttnTiles& g, void* scratch, hipStream_t s) {
+    return g.rows == 128 ? launch<T, EP, 4>(a, g, scratch, s) : launch<T, EP, 2>(a, g, scratch, s);
+}
+
+template <class T>
+int by_width(const krk_attention_args& a, const AttnTiles& g, void* scratch, hipStream_t s) {
+    if (a.E <= 32) return by_waves<T, 32>(a, g, scratch, s);
+    if (a.E <= 64) return by_waves<T, 64>(a, g, scratch, s);
+    if (a.E <= 96) return by_waves<T, 96>(a, g, scratch, s);
+    if (a.E <= 128) return by_waves<T, 128>(a, g, scratch, s);
+    return by_waves<T, 256>(a, g, scratch, s);
+}
+
+}  // namespace
+
+AttnTiles krk_attn_tiles(const krk_attention_args& a) {
+    AttnTiles g;
+    g.keys = a.type == KRK_TYPE_F32 ? 32 : 64;
+    g.rows = a.Tq > 256 ? 128 : 64;            // a block of 128 queries reads the keys half as often, but leaves more of it empty on short lines
+    const long blocks = (long)a.N * a.H * ((a.Tq + g.rows - 1) / g.rows), tiles = (a.Tk + g.keys - 1) / g.keys;
+    // few workgroups and a long axis: split it, eight tiles at least to each
+    g.splits = (int)max(1L, min(min((512 + blocks - 1) / max(blocks, 1L), tiles / 8), 64L));
+    g.range_bytes = a.documents ? (long)a.N * tiles * 8 : 0;
+    return g;
+}
+
+int krk_launch_attn_tiles(const krk_attention_args& a, const AttnTiles& g, void* scratch, hipStream_t s) {
+    return a.type == KRK_TYPE_F32 ? by_width<float>(a, g, scratch, s) : a.type == KRK_TYPE_BF16 ? by_width<bf16_t>(a, g, scratch, s) : by_width<f16_t>(a, g, scratch, s);
+}
