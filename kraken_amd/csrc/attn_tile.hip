@@ -23,12 +23,35 @@ __device__ __forceinline__ f32x16 mfma16(f16_t, const s16x8& a, const s16x8& b, 
 }
 __device__ __forceinline__ f32x16 mfma16(float, const s16x8&, const s16x8&, const f32x16& c) { return c; }
 
+// the lane 32 away: a query's keys lie in two lanes
+__device__ __forceinline__ float other_half_max(float v) {
+    const unsigned u = __builtin_bit_cast(unsigned, v);
+    const auto r = __builtin_amdgcn_permlane32_swap(u, u, false, false);
+    return fmaxf(__builtin_bit_cast(float, (unsigned)r[0]), __builtin_bit_cast(float, (unsigned)r[1]));
+}
+__device__ __forceinline__ float other_half_sum(float v) {
+    const unsigned u = __builtin_bit_cast(unsigned, v);
+    const auto r = __builtin_amdgcn_permlane32_swap(u, u, false, false);
+    return __builtin_bit_cast(float, (unsigned)r[0]) + __builtin_bit_cast(float, (unsigned)r[1]);
+}
+
 // exponent bits all ones: infinity or NaN
 template <class T> __device__ __forceinline__ bool odd_value(unsigned short v) {
     constexpr unsigned short M = sizeof(T) == 2 && __is_same(T, bf16_t) ? 0x7f80 : 0x7c00;
     return (v & M) == M;
 }
 __device__ __forceinline__ bool odd_float(float v) { return (__builtin_bit_cast(unsigned, v) & 0x7f800000u) == 0x7f800000u; }
+
+// the largest magnitude bits so far (both halves of a word apart), and whether one of them is odd
+template <class T> __device__ __forceinline__ unsigned odd_max(unsigned high, unsigned w) {
+    if constexpr (sizeof(T) == 4) return max(high, w & 0x7fffffffu);
+    typedef unsigned short u16x2 __attribute__((ext_vector_type(2)));
+    return __builtin_bit_cast(unsigned, __builtin_elementwise_max(__builtin_bit_cast(u16x2, high), __builtin_bit_cast(u16x2, w & 0x7fff7fffu)));
+}
+template <class T> __device__ __forceinline__ bool odd_found(unsigned high) {
+    if constexpr (sizeof(T) == 4) return high >= 0x7f800000u;
+    return odd_value<T>(high & 0xffff) || odd_value<T>(high >> 16);
+}
 
 // What an odd value does to a sum, as numbers a matrix product can count: 1 for NaN, 128 for +inf, 16384 for -inf; at most 64 keys of each in a
 // tile, so the counts stay apart and exact in fp32.
@@ -39,9 +62,9 @@ __device__ __forceinline__ float odd_sum(float count) {
     return nan || (pos && neg) ? __builtin_nanf("") : pos ? INFINITY : -INFINITY;
 }
 
-template <class T, int EP> struct Geo {
+template <class T, int EP, int NW> struct Geo {
     static constexpr bool F32 = sizeof(T) == 4;
-    static constexpr int BK = F32 ? 32 : 64;                              // keys of a tile
+    static constexpr int BK = F32 || NW < 4 ? 32 : 64;                    // keys of a tile
     static constexpr int SB = BK / 32, EB = EP / 32;
     static constexpr int KLD = F32 ? EP + 4 : EP + 8;                     // row pitches (elements) that spread a read over the banks:
     static constexpr int VLD = F32 ? EP + 8 : EP + (EP % 128 ? (EP % 64 ? 0 : 32) : 32);   // K rows by 16 bytes, V rows by quads of rows
@@ -63,15 +86,15 @@ __global__ __launch_bounds__(256) void attn_ranges_kernel(krk_attention_args a, 
 }
 
 template <class T, int EP, int NW>
-__global__ __launch_bounds__(NW * 64) void attn_tile_kernel(krk_attention_args a, int qblocks, int splits, int tiles, const int2* ranges) {
-    using G = Geo<T, EP>;
+__global__ __launch_bounds__(NW * 64, EP * sizeof(T) > 256 ? 1 : 2) void attn_tile_kernel(krk_attention_args a, int qblocks, int splits, int tiles, const int2* ranges) {
+    using G = Geo<T, EP, NW>;
     constexpr bool F32 = G::F32;
     constexpr int BK = G::BK, SB = G::SB, EB = G::EB, KLD = G::KLD, VLD = G::VLD, CV = G::CV, NT = NW * 64;
     constexpr int CPT = (G::CHUNKS + NT - 1) / NT, CPR = EP / CV;         // chunks per thread and per row
-    __shared__ __attribute__((aligned(16))) T Ks[BK * KLD];
-    __shared__ __attribute__((aligned(16))) T Vs[BK * VLD];
-    __shared__ int dks[BK];
-    __shared__ int odd[2];
+    __shared__ __attribute__((aligned(16))) T Kbuf[2][BK * KLD];
+    __shared__ __attribute__((aligned(16))) T Vbuf[2][BK * VLD];
+    __shared__ int dbuf[2][BK];
+    __shared__ int odd[4];
 
     // All query blocks and heads that share a key head run on one XCD (workgroups go round the eight of them), so its L2 holds their keys; the
     // blocks with the longest causal rows first.
@@ -199,208 +222,198 @@ __global__ __launch_bounds__(NW * 64) void attn_tile_kernel(krk_attention_args a
         if (docs && threadIdx.x < BK) dr = docs[min(t * BK + (int)threadIdx.x, a.Tk - 1)];
     };
 
-    if (threadIdx.x < 2) odd[threadIdx.x] = 0;
-    int tile = next(), turn = 0;
-    if (tile >= 0) fetch(tile);
-    while (tile >= 0) {
-        __syncthreads();                                                  // the tile before is used up
-        const int t = tile, k0 = t * BK;
-        // A value that is not finite must not reach the queries that may not see it: 0 x NaN is NaN.  Only tiles that some query of the workgroup
-        // sees in part can do that; they are searched while they go to LDS.
-        const bool search = k0 + BK > bmin || docs;
-        bool found = false;
+    // A value that is not finite must not reach the queries that may not see it: 0 x NaN is NaN.  Only tiles that some query of the workgroup sees
+    // in part can do that; they are searched while they go to LDS.
+    auto search = [&](int t) { return docs || (t + 1) * BK > bmin; };
+    auto put = [&](int t, int buf, int flag) {
+        unsigned high = 0;
 #pragma unroll
         for (int x = 0; x < CPT; ++x) {
             const int id = threadIdx.x + x * NT, row = id / CPR, e = (id - row * CPR) * CV;
             if (G::CHUNKS % NT == 0 || id < G::CHUNKS) {
-                *(u32x4*)&Ks[row * KLD + e] = kr[x];
-                *(u32x4*)&Vs[row * VLD + e] = vr[x];
-                if (search) {
+                *(u32x4*)&Kbuf[buf][row * KLD + e] = kr[x];
+                *(u32x4*)&Vbuf[buf][row * VLD + e] = vr[x];
 #pragma unroll
-                    for (int i = 0; i < 4; ++i) {
-                        const unsigned w = vr[x][i];
-                        if constexpr (F32) found |= odd_float(__builtin_bit_cast(float, w));
-                        else found |= odd_value<T>(w & 0xffff) || odd_value<T>(w >> 16);
-                    }
-                }
+                for (int i = 0; i < 4; ++i) high = odd_max<T>(high, vr[x][i]);
             }
         }
-        if (found) odd[turn & 1] = 1;
-        if (docs && threadIdx.x < BK) dks[threadIdx.x] = dr;
-        __syncthreads();
-        const bool bad = search && odd[turn & 1];
-        if (threadIdx.x == 0) odd[(turn + 1) & 1] = 0;
+        if (search(t) && odd_found<T>(high)) odd[flag] = 1;
+        if (docs && threadIdx.x < BK) dbuf[buf][threadIdx.x] = dr;
+    };
+
+    if (threadIdx.x < 4) odd[threadIdx.x] = 0;
+    __syncthreads();
+    int tile = next(), turn = 0;
+    if (tile >= 0) {
+        fetch(tile);
+        put(tile, 0, 0);
+    }
+    __syncthreads();
+    while (tile >= 0) {
+        const int t = tile, k0 = t * BK, buf = turn & 1;
+        const bool bad = search(t) && odd[turn & 3];
+        if (threadIdx.x == 0) odd[(turn + 2) & 3] = 0;                    // the flag that the next turn sets, read two turns ago
         ++turn;
         tile = next();
         if (tile >= 0) fetch(tile);
 
-        if (!awake || k0 >= wmax) continue;
-        bool part = k0 + BK > wmin;
-        if (docs) {
+        bool see = awake && k0 < wmax, part = k0 + BK > wmin;
+        if (docs && see) {
             const int2 r = ranges[(long)n * tiles + t];
-            if (r.x > whi || r.y < wlo) continue;
+            see = r.x <= whi && r.y >= wlo;
             part = part || r.x != r.y || wlo != whi;
         }
-
-        // S^T = K Q^T
-        f32x16 s[SB];
+        if (see) {
+            const T *Ks = Kbuf[buf], *Vs = Vbuf[buf];
 #pragma unroll
-        for (int b = 0; b < SB; ++b) {
+            for (int b = 0; b < SB; ++b) {
+                // S^T = K Q^T of 32 keys
+                f32x16 s;
 #pragma unroll
-            for (int i = 0; i < 16; ++i) s[b][i] = 0.f;
-            const T* kb = &Ks[(b * 32 + col) * KLD];
-            if constexpr (F32) {
-#pragma unroll
-                for (int g = 0; g < EP / 8; ++g) {
-                    const f32x4 k = *(const f32x4*)&kb[8 * g + 4 * half];
-#pragma unroll
-                    for (int i = 0; i < 4; ++i) s[b] = __builtin_amdgcn_mfma_f32_32x32x2f32(k[i], q32[g][i], s[b], 0, 0, 0);
-                }
-            } else {
-#pragma unroll
-                for (int ks = 0; ks < EP / 16; ++ks) s[b] = mfma16(T{}, *(const s16x8*)&kb[16 * ks + 8 * half], q16[ks], s[b]);
-            }
-        }
-        // register i of block b: key k0 + 32 b + 8 (i / 4) + 4 half + i % 4
-        float scale = c;
-        if (!plain) {
-            scale = 1.f;
-            const float d0 = (float)(mine.p - k0 - 4 * half);
-            if (a.cap > 0.f) {
+                for (int i = 0; i < 16; ++i) s[i] = 0.f;
+                const T* kb = &Ks[(b * 32 + col) * KLD];
                 if constexpr (F32) {
-                    const float raw = c * (1.f / LOG2E);
 #pragma unroll
-                    for (int b = 0; b < SB; ++b)
+                    for (int g = 0; g < EP / 8; ++g) {
+                        const f32x4 k = *(const f32x4*)&kb[8 * g + 4 * half];
 #pragma unroll
-                        for (int i = 0; i < 16; ++i) s[b][i] = seq_cap<T>(s[b][i] * raw, a.cap, rcap) * LOG2E;
-                } else {                                                  // cap tanh(x) = cap - 2 cap / (1 + e^2x): 2^-23 of cap off at most
-                    const float cl = a.cap * LOG2E, cx = 2.f * c * rcap;
+                        for (int i = 0; i < 4; ++i) s = __builtin_amdgcn_mfma_f32_32x32x2f32(k[i], q32[g][i], s, 0, 0, 0);
+                    }
+                } else {
 #pragma unroll
-                    for (int b = 0; b < SB; ++b)
-#pragma unroll
-                        for (int i = 0; i < 16; ++i)
-                            s[b][i] = __builtin_fmaf(-2.f * cl, __builtin_amdgcn_rcpf(1.f + __builtin_amdgcn_exp2f(s[b][i] * cx)), cl);
+                    for (int ks = 0; ks < EP / 16; ++ks) s = mfma16(T{}, *(const s16x8*)&kb[16 * ks + 8 * half], q16[ks], s);
                 }
-            } else {
+                // register i: key k0 + 32 b + 8 (i / 4) + 4 half + i % 4
+                float scale = c;
+                if (!plain) {
+                    scale = 1.f;
+                    if (a.cap > 0.f) {
+                        if constexpr (F32) {
+                            const float raw = c * (1.f / LOG2E);
 #pragma unroll
-                for (int b = 0; b < SB; ++b)
+                            for (int i = 0; i < 16; ++i) s[i] = seq_cap<T>(s[i] * raw, a.cap, rcap) * LOG2E;
+                        } else {                                          // cap tanh(x) = cap - 2 cap / (1 + e^2x): 2^-23 of cap off at most
+                            const float cl = a.cap * LOG2E, cx = 2.f * c * rcap;
 #pragma unroll
-                    for (int i = 0; i < 16; ++i) s[b][i] *= c;
-            }
-            if (a.slopes)
+                            for (int i = 0; i < 16; ++i)
+                                s[i] = __builtin_fmaf(-2.f * cl, __builtin_amdgcn_rcpf(1.f + __builtin_amdgcn_exp2f(s[i] * cx)), cl);
+                        }
+                    } else {
 #pragma unroll
-                for (int b = 0; b < SB; ++b)
+                        for (int i = 0; i < 16; ++i) s[i] *= c;
+                    }
+                    if (a.slopes) {
+                        const float d0 = (float)(mine.p - k0 - 32 * b - 4 * half);
 #pragma unroll
-                    for (int i = 0; i < 16; ++i)
-                        s[b][i] = __builtin_fmaf(-slope, fabsf(d0 - (float)(32 * b + 8 * (i / 4) + i % 4)), s[b][i]);
-        }
-        if (part) {
-            const int room = lim - k0 - 4 * half;
-#pragma unroll
-            for (int b = 0; b < SB; ++b)
-#pragma unroll
-                for (int i = 0; i < 16; ++i) {
-                    const int x = 32 * b + 8 * (i / 4) + i % 4;
-                    bool ok = x < room;
-                    if (docs) ok = ok && dks[x + 4 * half] == doc;
-                    s[b][i] = ok ? s[b][i] : -INFINITY;
+                        for (int i = 0; i < 16; ++i) s[i] = __builtin_fmaf(-slope, fabsf(d0 - (float)(8 * (i / 4) + i % 4)), s[i]);
+                    }
                 }
-        }
-        float top = s[0][0];
-#pragma unroll
-        for (int b = 0; b < SB; ++b)
-#pragma unroll
-            for (int i = 0; i < 16; ++i) top = fmaxf(top, s[b][i]);
-        top = fmaxf(top, __shfl_xor(top, 32)) * scale;
-        // The reference point moves only when a score passes it by 2^8: weights up to 256 are as exact, and most tiles leave the sums alone.
-        if (__ballot(top > m + 8.f)) {
-            const float nm = fmaxf(m, top), f = __builtin_amdgcn_exp2f(m - (nm == -INFINITY ? 0.f : nm));
-            m = nm;
-            l *= f;
-#pragma unroll
-            for (int eb = 0; eb < EB; ++eb)
-#pragma unroll
-                for (int i = 0; i < 16; ++i) o[eb][i] *= f;
-        }
-        const float ref = m == -INFINITY ? 0.f : m;
-        float sum = 0.f;
-#pragma unroll
-        for (int b = 0; b < SB; ++b)
-#pragma unroll
-            for (int i = 0; i < 16; ++i) {
-                s[b][i] = __builtin_amdgcn_exp2f(__builtin_fmaf(s[b][i], scale, -ref));
-                sum += s[b][i];
-            }
-        l += sum;
-
-        // O^T += V^T P^T
-        if constexpr (F32) {
-#pragma unroll
-            for (int eb = 0; eb < EB; ++eb) {
-                f32x16 marks;
-                if (bad)
-#pragma unroll
-                    for (int i = 0; i < 16; ++i) marks[i] = 0.f;
-#pragma unroll
-                for (int b = 0; b < SB; ++b)
+                if (part) {
+                    const int room = lim - k0 - 32 * b - 4 * half;
 #pragma unroll
                     for (int i = 0; i < 16; ++i) {
-                        float v = Vs[(b * 32 + 8 * (i / 4) + i % 4 + 4 * half) * VLD + eb * 32 + col];
+                        const int x = 8 * (i / 4) + i % 4;
+                        bool ok = x < room;
+                        if (docs) ok = ok && dbuf[buf][32 * b + x + 4 * half] == doc;
+                        s[i] = ok ? s[i] : -INFINITY;
+                    }
+                }
+                float top = s[0];
+#pragma unroll
+                for (int i = 1; i < 16; ++i) top = fmaxf(top, s[i]);
+                top = other_half_max(top) * scale;
+                // The reference point moves only when a score passes it by 2^8: weights up to 256 are as exact, and most tiles leave the sums alone.
+                if (__ballot(top > m + 8.f)) {
+                    const float nm = fmaxf(m, top), f = __builtin_amdgcn_exp2f(m - (nm == -INFINITY ? 0.f : nm));
+                    m = nm;
+                    l *= f;
+#pragma unroll
+                    for (int eb = 0; eb < EB; ++eb)
+#pragma unroll
+                        for (int i = 0; i < 16; ++i) o[eb][i] *= f;
+                }
+                const float ref = m == -INFINITY ? 0.f : m;
+                float sum = 0.f;
+#pragma unroll
+                for (int i = 0; i < 16; ++i) {
+                    s[i] = __builtin_amdgcn_exp2f(__builtin_fmaf(s[i], scale, -ref));
+                    sum += s[i];
+                }
+                l += sum;
+
+                // O^T += V^T P^T
+                if constexpr (F32) {
+#pragma unroll
+                    for (int eb = 0; eb < EB; ++eb) {
+                        const T* vb = &Vs[(b * 32 + 4 * half) * VLD + eb * 32 + col];
+                        if (!bad) {
+#pragma unroll
+                            for (int i = 0; i < 16; ++i)
+                                o[eb] = __builtin_amdgcn_mfma_f32_32x32x2f32(vb[(8 * (i / 4) + i % 4) * VLD], s[i], o[eb], 0, 0, 0);
+                        } else {
+                            f32x16 marks;
+#pragma unroll
+                            for (int i = 0; i < 16; ++i) marks[i] = 0.f;
+#pragma unroll
+                            for (int i = 0; i < 16; ++i) {
+                                const float v = vb[(8 * (i / 4) + i % 4) * VLD];
+                                const bool is = odd_float(v);
+                                marks = __builtin_amdgcn_mfma_f32_32x32x2f32(is ? odd_mark(v) : 0.f, s[i] > 0.f ? 1.f : s[i], marks, 0, 0, 0);
+                                o[eb] = __builtin_amdgcn_mfma_f32_32x32x2f32(is ? 0.f : v, s[i], o[eb], 0, 0, 0);
+                            }
+#pragma unroll
+                            for (int i = 0; i < 16; ++i) o[eb][i] += odd_sum(marks[i]);
+                        }
+                    }
+                } else {
+                    s16x8 p[2];
+#pragma unroll
+                    for (int x = 0; x < 2; ++x)
+#pragma unroll
+                        for (int i = 0; i < 8; ++i) p[x][i] = __builtin_bit_cast(short, from_f<T>(s[8 * x + i]));
+                    // lane l gets, for channel l % 32, the four keys of its half: 16 lanes hold four rows of 16 channels, read transposed
+                    const T* vb = &Vs[(32 * b + 4 * half + (col & 15) / 4) * VLD + 16 * (col >> 4) + 4 * (col & 3)];
+#pragma unroll
+                    for (int eb = 0; eb < EB; ++eb) {
+                        s16x8 v[2];
+#pragma unroll
+                        for (int x = 0; x < 2; ++x) {
+                            typedef __attribute__((address_space(3))) s16x4 lds4;
+                            const s16x4 lo = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds4*)&vb[16 * x * VLD + eb * 32]);
+                            const s16x4 hi = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds4*)&vb[(16 * x + 8) * VLD + eb * 32]);
+                            v[x] = __builtin_shufflevector(lo, hi, 0, 1, 2, 3, 4, 5, 6, 7);
+                        }
                         if (bad) {
-                            const bool is = odd_float(v);
-                            marks = __builtin_amdgcn_mfma_f32_32x32x2f32(is ? odd_mark(v) : 0.f, s[b][i] > 0.f ? 1.f : s[b][i], marks, 0, 0, 0);
-                            v = is ? 0.f : v;
+                            f32x16 marks;
+#pragma unroll
+                            for (int i = 0; i < 16; ++i) marks[i] = 0.f;
+#pragma unroll
+                            for (int x = 0; x < 2; ++x) {
+                                s16x8 mark, one;
+#pragma unroll
+                                for (int i = 0; i < 8; ++i) {
+                                    const bool is = odd_value<T>((unsigned short)v[x][i]);
+                                    mark[i] = __builtin_bit_cast(short, from_f<T>(is ? odd_mark(to_f(__builtin_bit_cast(T, v[x][i]))) : 0.f));
+                                    const float w = s[8 * x + i];
+                                    one[i] = __builtin_bit_cast(short, from_f<T>(w > 0.f ? 1.f : w));
+                                    if (is) v[x][i] = 0;
+                                }
+                                marks = mfma16(T{}, mark, one, marks);
+                            }
+#pragma unroll
+                            for (int i = 0; i < 16; ++i) o[eb][i] += odd_sum(marks[i]);
                         }
-                        o[eb] = __builtin_amdgcn_mfma_f32_32x32x2f32(v, s[b][i], o[eb], 0, 0, 0);
+#pragma unroll
+                        for (int x = 0; x < 2; ++x) o[eb] = mfma16(T{}, v[x], p[x], o[eb]);
                     }
-                if (bad)
-#pragma unroll
-                    for (int i = 0; i < 16; ++i) o[eb][i] += odd_sum(marks[i]);
-            }
-        } else {
-            s16x8 p[SB * 2];
-#pragma unroll
-            for (int x = 0; x < SB * 2; ++x)
-#pragma unroll
-                for (int i = 0; i < 8; ++i) p[x][i] = __builtin_bit_cast(short, from_f<T>(s[x / 2][8 * (x & 1) + i]));
-            const int vrow = 4 * half + (col & 15) / 4, vcol = 16 * (col >> 4) + 4 * (col & 3);
-#pragma unroll
-            for (int eb = 0; eb < EB; ++eb) {
-                s16x8 v[SB * 2];
-#pragma unroll
-                for (int x = 0; x < SB * 2; ++x) {
-                    typedef __attribute__((address_space(3))) s16x4 lds4;
-                    const s16x4 lo = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds4*)&Vs[(16 * x + vrow) * VLD + eb * 32 + vcol]);
-                    const s16x4 hi = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds4*)&Vs[(16 * x + 8 + vrow) * VLD + eb * 32 + vcol]);
-                    v[x] = __builtin_shufflevector(lo, hi, 0, 1, 2, 3, 4, 5, 6, 7);
                 }
-                if (bad) {
-                    f32x16 marks;
-#pragma unroll
-                    for (int i = 0; i < 16; ++i) marks[i] = 0.f;
-#pragma unroll
-                    for (int x = 0; x < SB * 2; ++x) {
-                        s16x8 mark, one;
-#pragma unroll
-                        for (int i = 0; i < 8; ++i) {
-                            const bool is = odd_value<T>((unsigned short)v[x][i]);
-                            mark[i] = __builtin_bit_cast(short, from_f<T>(is ? odd_mark(to_f(__builtin_bit_cast(T, v[x][i]))) : 0.f));
-                            const float w = s[x / 2][8 * (x & 1) + i];
-                            one[i] = __builtin_bit_cast(short, from_f<T>(w > 0.f ? 1.f : w));
-                            if (is) v[x][i] = 0;
-                        }
-                        marks = mfma16(T{}, mark, one, marks);
-                    }
-#pragma unroll
-                    for (int i = 0; i < 16; ++i) o[eb][i] += odd_sum(marks[i]);
-                }
-#pragma unroll
-                for (int x = 0; x < SB * 2; ++x) o[eb] = mfma16(T{}, v[x], p[x], o[eb]);
             }
         }
+        if (tile >= 0) put(tile, buf ^ 1, turn & 3);                      // last read a turn ago, behind the barrier
+        __syncthreads();
     }
 
-    l += __shfl_xor(l, 32);
+    l = other_half_sum(l);
     if (qi >= a.Tq) return;
     if (splits == 1) {
         const float r = lim > 0 && l != 0.f ? 1.f / l : 0.f;
@@ -452,7 +465,9 @@ int launch(const krk_attention_args& a, const AttnTiles& g, void* scratch, hipSt
 
 template <class T, int EP>
 int by_waves(const krk_attention_args& a, const AttnTiles& g, void* scratch, hipStream_t s) {
-    return g.rows == 128 ? launch<T, EP, 4>(a, g, scratch, s) : launch<T, EP, 2>(a, g, scratch, s);
+    if constexpr (EP * sizeof(T) <= 256)
+        if (g.rows == 64) return launch<T, EP, 2>(a, g, scratch, s);
+    return launch<T, EP, 4>(a, g, scratch, s);
 }
 
 template <class T>
@@ -468,8 +483,10 @@ int by_width(const krk_attention_args& a, const AttnTiles& g, void* scratch, hip
 
 AttnTiles krk_attn_tiles(const krk_attention_args& a) {
     AttnTiles g;
-    g.keys = a.type == KRK_TYPE_F32 ? 32 : 64;
-    g.rows = a.Tq > 256 ? 128 : 64;            // a block of 128 queries reads the keys half as often, but leaves more of it empty on short lines
+    // a block of 128 queries reads the keys half as often, but leaves more of it empty on short lines; wide heads have no registers for 64
+    const bool f32 = a.type == KRK_TYPE_F32;
+    g.rows = a.Tq > 256 || a.E > (f32 ? 64 : 128) ? 128 : 64;
+    g.keys = f32 || g.rows == 64 ? 32 : 64;
     const long blocks = (long)a.N * a.H * ((a.Tq + g.rows - 1) / g.rows), tiles = (a.Tk + g.keys - 1) / g.keys;
     // few workgroups and a long axis: split it, eight tiles at least to each
     g.splits = (int)max(1L, min(min((512 + blocks - 1) / max(blocks, 1L), tiles / 8), 64L));
