@@ -199,8 +199,9 @@ int by_rows(const krk_attention_args& a, hipStream_t s) {
     }
 }
 
-// One or two query positions read the keys as often as they are rows; more of them go to the tile kernel, which reads them once per block.
-bool by_tiles(const krk_attention_args& a) { return a.Tq > 2; }
+// One or two query positions read the keys as often as they are rows; more of them go to the tile kernel, which reads them once per block.  Heads of
+// less than 16 bytes stay here: the tile kernel's loads are 16 bytes within a row.
+bool by_tiles(const krk_attention_args& a) { return a.Tq > 2 && a.E * (a.type == KRK_TYPE_F32 ? 4 : 2) >= 16; }
 
 long part_bytes(const krk_attention_args& a, int splits) {
     return splits == 1 ? 0 : ((long)a.N * a.Tq * a.H * splits * (a.E + 2) * (long)sizeof(float) + 15) / 16 * 16;

@@ -23,11 +23,33 @@ __device__ __forceinline__ f32x16 mfma16(f16_t, const s16x8& a, const s16x8& b, 
 }
 __device__ __forceinline__ f32x16 mfma16(float, const s16x8&, const s16x8&, const f32x16& c) { return c; }
 
+// The 16 bytes of a head from channel e on, zeros behind its end (E channels, 16 bytes at least).  The last, partial one is loaded so that it ENDS
+// there: one load without a condition whatever E is, and none past the row; place_chunk moves it into place, apart from the load, so that
+// nothing waits for the load before it has to.
+typedef unsigned long long u64x2 __attribute__((ext_vector_type(2)));
+template <class T> __device__ __forceinline__ u32x4 load_chunk(const T* row, int e, int E) {
+    u32x4 r;
+    __builtin_memcpy(&r, row + min(e, E - VecOf<T>::V), 16);
+    return r;
+}
+template <class T> __device__ __forceinline__ u32x4 place_chunk(u32x4 r, int e, int E) {
+    const int sh = max(0, (e + VecOf<T>::V - E) * (int)sizeof(T) * 8);
+    u64x2 w = __builtin_bit_cast(u64x2, r);
+    w[0] = sh >= 64 ? w[1] >> (sh & 63) : sh ? w[0] >> sh | w[1] << (64 - sh) : w[0];
+    w[1] = sh >= 64 ? 0 : w[1] >> sh;
+    if (sh >= 128) w[0] = 0;
+    return __builtin_bit_cast(u32x4, w);
+}
+
 // the lane 32 away: a query's keys lie in two lanes
 __device__ __forceinline__ float other_half_max(float v) {
     const unsigned u = __builtin_bit_cast(unsigned, v);
     const auto r = __builtin_amdgcn_permlane32_swap(u, u, false, false);
     return fmaxf(__builtin_bit_cast(float, (unsigned)r[0]), __builtin_bit_cast(float, (unsigned)r[1]));
+}
+__device__ __forceinline__ unsigned other_half_or(unsigned u) {
+    const auto r = __builtin_amdgcn_permlane32_swap(u, u, false, false);
+    return (unsigned)r[0] | (unsigned)r[1];
 }
 __device__ __forceinline__ float other_half_sum(float v) {
     const unsigned u = __builtin_bit_cast(unsigned, v);
@@ -51,15 +73,6 @@ template <class T> __device__ __forceinline__ unsigned odd_max(unsigned high, un
 template <class T> __device__ __forceinline__ bool odd_found(unsigned high) {
     if constexpr (sizeof(T) == 4) return high >= 0x7f800000u;
     return odd_value<T>(high & 0xffff) || odd_value<T>(high >> 16);
-}
-
-// What an odd value does to a sum, as numbers a matrix product can count: 1 for NaN, 128 for +inf, 16384 for -inf; at most 64 keys of each in a
-// tile, so the counts stay apart and exact in fp32.
-__device__ __forceinline__ float odd_mark(float v) { return v != v ? 1.f : v > 0.f ? 128.f : 16384.f; }
-__device__ __forceinline__ float odd_sum(float count) {
-    const int c = (int)count, nan = c & 127, pos = (c >> 7) & 127, neg = c >> 14;
-    if (c == 0) return 0.f;
-    return nan || (pos && neg) ? __builtin_nanf("") : pos ? INFINITY : -INFINITY;
 }
 
 template <class T, int EP, int NW> struct Geo {
@@ -86,23 +99,25 @@ __global__ __launch_bounds__(256) void attn_ranges_kernel(krk_attention_args a, 
 }
 
 template <class T, int EP, int NW>
-__global__ __launch_bounds__(NW * 64, EP * sizeof(T) > 256 ? 1 : 2) void attn_tile_kernel(krk_attention_args a, int qblocks, int splits, int tiles, const int2* ranges) {
+__global__ __launch_bounds__(NW * 64, EP * sizeof(T) > 256 ? 1 : sizeof(T) == 2 && EP <= 64 ? 3 : 2) void attn_tile_kernel(krk_attention_args a, int qblocks, int cut, int splits, int tiles, const int2* ranges) {
     using G = Geo<T, EP, NW>;
     constexpr bool F32 = G::F32;
     constexpr int BK = G::BK, SB = G::SB, EB = G::EB, KLD = G::KLD, VLD = G::VLD, CV = G::CV, NT = NW * 64;
     constexpr int CPT = (G::CHUNKS + NT - 1) / NT, CPR = EP / CV;         // chunks per thread and per row
     __shared__ __attribute__((aligned(16))) T Kbuf[2][BK * KLD];
     __shared__ __attribute__((aligned(16))) T Vbuf[2][BK * VLD];
-    __shared__ int dbuf[2][BK];
+    __shared__ __attribute__((aligned(16))) int dbuf[2][BK];
     __shared__ int odd[4];
+    __shared__ unsigned infs[2][2][SB][EP];                               // where the tile's odd values were: +inf / -inf (NaN: both), a bit per key
 
-    // All query blocks and heads that share a key head run on one XCD (workgroups go round the eight of them), so its L2 holds their keys; the
-    // blocks with the longest causal rows first.
-    const int rep = a.H / a.Hk, inner = qblocks * rep;
-    const long id = blockIdx.x / 8;
-    const long kvh = (blockIdx.x & 7) + 8 * (id / inner);
-    if (kvh >= (long)a.N * a.Hk) return;
-    const int n = kvh / a.Hk, hk = kvh % a.Hk, in = id % inner;
+    // All query blocks and heads that share a key head run on one XCD (workgroups go round the eight of them), so its L2 holds their keys; where
+    // the key heads do not go round evenly each is cut into `cut` interleaved parts.  The blocks with the longest causal rows come first.
+    const int rep = a.H / a.Hk, inner = qblocks * rep, part_size = (inner + cut - 1) / cut;
+    const long id = blockIdx.x / 8, group = (blockIdx.x & 7) + 8 * (id / part_size);
+    const int in = (int)(id % part_size) * cut + (int)(group % cut);
+    if (in >= inner) return;
+    const long kvh = group / cut;
+    const int n = kvh / a.Hk, hk = kvh % a.Hk;
     const int h = hk * rep + in % rep, q0 = (qblocks - 1 - in / rep) * NW * 32;
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), half = lane >> 5, col = lane & 31;
     const int qlen = seq_len(a.q_lens, n, a.Tq), split = blockIdx.y;
@@ -111,6 +126,7 @@ __global__ __launch_bounds__(NW * 64, EP * sizeof(T) > 256 ? 1 : 2) void attn_ti
     const int* docs = a.documents ? a.documents + n * a.doc_n : nullptr;
 
     // what the masks say: about this lane's query, about the wave's first (the shortest reach) and last one, about the workgroup
+    const int klen = seq_len(a.k_lens, n, a.Tk);
     const AttnRow mine = query_row(a, n, min(qi, a.Tq - 1));
     const int lim = qi < qlen ? mine.limit : 0;
     const int wfirst = q0 + wave * 32, wlast = min(wfirst + 31, qlen - 1);
@@ -142,21 +158,19 @@ __global__ __launch_bounds__(NW * 64, EP * sizeof(T) > 256 ? 1 : 2) void attn_ti
     f32x4 q32[F32 ? EP / 8 : 1];
     {
         const T* qp = (const T*)a.q + n * a.q_n + (long)min(qi, a.Tq - 1) * a.q_t + h * a.q_h;
-        if constexpr (F32) {
+        constexpr int NQ = F32 ? EP / 8 : EP / 16, STEP = F32 ? 8 : 16;
+        u32x4 raw[NQ];
 #pragma unroll
-            for (int g = 0; g < EP / 8; ++g) {
-                float v[4];
-                load_vec<float, 4>(qp + 8 * g + 4 * half, a.E - 8 * g - 4 * half, v);
+        for (int x = 0; x < NQ; ++x) raw[x] = load_chunk<T>(qp, STEP * x + STEP / 2 * half, a.E);
 #pragma unroll
-                for (int i = 0; i < 4; ++i) q32[g][i] = v[i] * sign;
-            }
-        } else {
+        for (int x = 0; x < NQ; ++x) {
+            if (a.E != EP) raw[x] = place_chunk<T>(raw[x], STEP * x + STEP / 2 * half, a.E);
+            if constexpr (F32) q32[x] = __builtin_bit_cast(f32x4, raw[x]) * sign;
+            else {
+                q16[x] = __builtin_bit_cast(s16x8, raw[x]);
+                if (a.scale <= 0.f)
 #pragma unroll
-            for (int ks = 0; ks < EP / 16; ++ks) {
-                float v[8];
-                load_vec<T, 8>(qp + 16 * ks + 8 * half, a.E - 16 * ks - 8 * half, v);
-#pragma unroll
-                for (int i = 0; i < 8; ++i) q16[ks][i] = __builtin_bit_cast(short, from_f<T>(v[i] * sign));
+                    for (int i = 0; i < 8; ++i) q16[x][i] = __builtin_bit_cast(short, from_f<T>(to_f(__builtin_bit_cast(T, q16[x][i])) * sign));
             }
         }
     }
@@ -177,6 +191,7 @@ __global__ __launch_bounds__(NW * 64, EP * sizeof(T) > 256 ? 1 : 2) void attn_ti
     const int t1 = min(want, (split + 1) * span);
     int base = split * span - 64;
     unsigned long long left = 0;
+    int2 here = make_int2(0, 0), now = make_int2(0, 0);                   // id ranges: of the tile that this lane looked at, of the one taken
     auto next = [&]() -> int {
         while (!left) {
             base += 64;
@@ -184,13 +199,14 @@ __global__ __launch_bounds__(NW * 64, EP * sizeof(T) > 256 ? 1 : 2) void attn_ti
             const int t = base + lane;
             bool in = t < t1;
             if (docs && in) {
-                const int2 r = ranges[(long)n * tiles + t];
-                in = r.x <= bhi && r.y >= blo;
+                here = ranges[(long)n * tiles + t];
+                in = here.x <= bhi && here.y >= blo;
             }
             left = __ballot(in);
         }
         const int b = __builtin_ctzll(left);
         left &= left - 1;
+        now = make_int2(__builtin_amdgcn_readlane(here.x, b), __builtin_amdgcn_readlane(here.y, b));
         return base + b;
     };
 
@@ -198,74 +214,90 @@ __global__ __launch_bounds__(NW * 64, EP * sizeof(T) > 256 ? 1 : 2) void attn_ti
     const T* vp = (const T*)a.v + n * a.v_n + hk * a.v_h;
     u32x4 kr[CPT], vr[CPT];
     int dr = 0;
-    auto fetch = [&](int t) {
+    auto fetch = [&](int t) {                                             // rows behind the last valid key repeat it: they are masked
 #pragma unroll
         for (int x = 0; x < CPT; ++x) {
             const int id = threadIdx.x + x * NT, row = id / CPR, e = (id - row * CPR) * CV;
-            const int j = t * BK + row;
-            kr[x] = vr[x] = (u32x4){0, 0, 0, 0};
-            if ((G::CHUNKS % NT == 0 || id < G::CHUNKS) && j < mine.klen) {
-                const T *ks = kp + (long)j * a.k_t + e, *vs = vp + (long)j * a.v_t + e;
-                if (e + CV <= a.E) {
-                    __builtin_memcpy(&kr[x], ks, 16);
-                    __builtin_memcpy(&vr[x], vs, 16);
-                } else if (e < a.E) {
-                    T kt[CV] = {}, vt[CV] = {};
-#pragma unroll
-                    for (int i = 0; i < CV; ++i)
-                        if (e + i < a.E) kt[i] = ks[i], vt[i] = vs[i];
-                    __builtin_memcpy(&kr[x], kt, 16);
-                    __builtin_memcpy(&vr[x], vt, 16);
-                }
-            }
+            const int j = min(t * BK + (G::CHUNKS % NT == 0 ? row : min(row, BK - 1)), klen - 1);
+            kr[x] = load_chunk<T>(kp + (long)j * a.k_t, e, a.E);
+            vr[x] = load_chunk<T>(vp + (long)j * a.v_t, e, a.E);
         }
-        if (docs && threadIdx.x < BK) dr = docs[min(t * BK + (int)threadIdx.x, a.Tk - 1)];
+        if (docs && threadIdx.x < BK) dr = docs[min(t * BK + (int)threadIdx.x, klen - 1)];
     };
 
     // A value that is not finite must not reach the queries that may not see it: 0 x NaN is NaN.  Only tiles that some query of the workgroup sees
     // in part can do that; they are searched while they go to LDS.
     auto search = [&](int t) { return docs || (t + 1) * BK > bmin; };
-    auto put = [&](int t, int buf, int flag) {
+    auto put = [&](int t, int buf, int turn) {
         unsigned high = 0;
+        if (a.E != EP)
+#pragma unroll
+            for (int x = 0; x < CPT; ++x) {
+                const int e = (threadIdx.x + x * NT) % CPR * CV;
+                kr[x] = place_chunk<T>(kr[x], e, a.E);
+                vr[x] = place_chunk<T>(vr[x], e, a.E);
+            }
+#pragma unroll
+        for (int x = 0; x < CPT; ++x)
+#pragma unroll
+            for (int i = 0; i < 4; ++i) high = odd_max<T>(high, vr[x][i]);
+        const bool hit = search(t) && odd_found<T>(high);
+        if (hit) odd[turn & 3] = 1;
 #pragma unroll
         for (int x = 0; x < CPT; ++x) {
             const int id = threadIdx.x + x * NT, row = id / CPR, e = (id - row * CPR) * CV;
             if (G::CHUNKS % NT == 0 || id < G::CHUNKS) {
                 *(u32x4*)&Kbuf[buf][row * KLD + e] = kr[x];
                 *(u32x4*)&Vbuf[buf][row * VLD + e] = vr[x];
-#pragma unroll
-                for (int i = 0; i < 4; ++i) high = odd_max<T>(high, vr[x][i]);
+                if (hit)                                                  // its own elements again, one by one
+                    for (int i = 0; i < CV; ++i) {
+                        const float v = to_f<T>(Vbuf[buf][row * VLD + e + i]);
+                        if (!odd_float(v)) continue;
+                        if (!(v < 0.f)) atomicOr(&infs[buf][0][row >> 5][e + i], 1u << (row & 31));
+                        if (!(v > 0.f)) atomicOr(&infs[buf][1][row >> 5][e + i], 1u << (row & 31));
+                        Vbuf[buf][row * VLD + e + i] = from_f<T>(0.f);
+                    }
             }
         }
-        if (search(t) && odd_found<T>(high)) odd[flag] = 1;
         if (docs && threadIdx.x < BK) dbuf[buf][threadIdx.x] = dr;
     };
+    auto clear = [&](int buf) {
+        for (int i = threadIdx.x; i < 2 * SB * EP; i += NT) (&infs[buf][0][0][0])[i] = 0;
+    };
 
+    for (int x = 0; x < 2; ++x) clear(x);
     if (threadIdx.x < 4) odd[threadIdx.x] = 0;
     __syncthreads();
     int tile = next(), turn = 0;
+    bool was = false;
     if (tile >= 0) {
         fetch(tile);
         put(tile, 0, 0);
     }
+    __builtin_amdgcn_s_waitcnt(0x0f70);                                   // vmcnt(0): nothing of the prologue is waited for behind the loop's own loads
     __syncthreads();
     while (tile >= 0) {
         const int t = tile, k0 = t * BK, buf = turn & 1;
+        const int2 r = now;
         const bool bad = search(t) && odd[turn & 3];
         if (threadIdx.x == 0) odd[(turn + 2) & 3] = 0;                    // the flag that the next turn sets, read two turns ago
+        if (was) {                                                        // the places that the next tile's go to, read in the last turn
+            clear(buf ^ 1);
+            __syncthreads();
+        }
+        was = bad;
         ++turn;
         tile = next();
         if (tile >= 0) fetch(tile);
 
         bool see = awake && k0 < wmax, part = k0 + BK > wmin;
         if (docs && see) {
-            const int2 r = ranges[(long)n * tiles + t];
             see = r.x <= whi && r.y >= wlo;
             part = part || r.x != r.y || wlo != whi;
         }
         if (see) {
             const T *Ks = Kbuf[buf], *Vs = Vbuf[buf];
-#pragma unroll
+#pragma unroll 1
             for (int b = 0; b < SB; ++b) {
                 // S^T = K Q^T of 32 keys
                 f32x16 s;
@@ -311,11 +343,13 @@ __global__ __launch_bounds__(NW * 64, EP * sizeof(T) > 256 ? 1 : 2) void attn_ti
                 if (part) {
                     const int room = lim - k0 - 32 * b - 4 * half;
 #pragma unroll
-                    for (int i = 0; i < 16; ++i) {
-                        const int x = 8 * (i / 4) + i % 4;
-                        bool ok = x < room;
-                        if (docs) ok = ok && dbuf[buf][32 * b + x + 4 * half] == doc;
-                        s[i] = ok ? s[i] : -INFINITY;
+                    for (int i = 0; i < 16; ++i) s[i] = 8 * (i / 4) + i % 4 < room ? s[i] : -INFINITY;
+                    if (docs) {
+                        int4 ids[4];
+#pragma unroll
+                        for (int g = 0; g < 4; ++g) ids[g] = *(const int4*)&dbuf[buf][32 * b + 8 * g + 4 * half];
+#pragma unroll
+                        for (int i = 0; i < 16; ++i) s[i] = (&ids[i / 4].x)[i % 4] == doc ? s[i] : -INFINITY;
                     }
                 }
                 float top = s[0];
@@ -342,29 +376,18 @@ __global__ __launch_bounds__(NW * 64, EP * sizeof(T) > 256 ? 1 : 2) void attn_ti
                 l += sum;
 
                 // O^T += V^T P^T
+                unsigned seen = 0;                                        // of this half's keys, those with a weight
                 if constexpr (F32) {
 #pragma unroll
                     for (int eb = 0; eb < EB; ++eb) {
                         const T* vb = &Vs[(b * 32 + 4 * half) * VLD + eb * 32 + col];
-                        if (!bad) {
 #pragma unroll
-                            for (int i = 0; i < 16; ++i)
-                                o[eb] = __builtin_amdgcn_mfma_f32_32x32x2f32(vb[(8 * (i / 4) + i % 4) * VLD], s[i], o[eb], 0, 0, 0);
-                        } else {
-                            f32x16 marks;
-#pragma unroll
-                            for (int i = 0; i < 16; ++i) marks[i] = 0.f;
-#pragma unroll
-                            for (int i = 0; i < 16; ++i) {
-                                const float v = vb[(8 * (i / 4) + i % 4) * VLD];
-                                const bool is = odd_float(v);
-                                marks = __builtin_amdgcn_mfma_f32_32x32x2f32(is ? odd_mark(v) : 0.f, s[i] > 0.f ? 1.f : s[i], marks, 0, 0, 0);
-                                o[eb] = __builtin_amdgcn_mfma_f32_32x32x2f32(is ? 0.f : v, s[i], o[eb], 0, 0, 0);
-                            }
-#pragma unroll
-                            for (int i = 0; i < 16; ++i) o[eb][i] += odd_sum(marks[i]);
-                        }
+                        for (int i = 0; i < 16; ++i)
+                            o[eb] = __builtin_amdgcn_mfma_f32_32x32x2f32(vb[(8 * (i / 4) + i % 4) * VLD], s[i], o[eb], 0, 0, 0);
                     }
+                    if (bad)
+#pragma unroll
+                        for (int i = 0; i < 16; ++i) seen |= s[i] != 0.f ? 1u << (8 * (i / 4) + i % 4) : 0u;
                 } else {
                     s16x8 p[2];
 #pragma unroll
@@ -383,33 +406,27 @@ __global__ __launch_bounds__(NW * 64, EP * sizeof(T) > 256 ? 1 : 2) void attn_ti
                             const s16x4 hi = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds4*)&vb[(16 * x + 8) * VLD + eb * 32]);
                             v[x] = __builtin_shufflevector(lo, hi, 0, 1, 2, 3, 4, 5, 6, 7);
                         }
-                        if (bad) {
-                            f32x16 marks;
-#pragma unroll
-                            for (int i = 0; i < 16; ++i) marks[i] = 0.f;
-#pragma unroll
-                            for (int x = 0; x < 2; ++x) {
-                                s16x8 mark, one;
-#pragma unroll
-                                for (int i = 0; i < 8; ++i) {
-                                    const bool is = odd_value<T>((unsigned short)v[x][i]);
-                                    mark[i] = __builtin_bit_cast(short, from_f<T>(is ? odd_mark(to_f(__builtin_bit_cast(T, v[x][i]))) : 0.f));
-                                    const float w = s[8 * x + i];
-                                    one[i] = __builtin_bit_cast(short, from_f<T>(w > 0.f ? 1.f : w));
-                                    if (is) v[x][i] = 0;
-                                }
-                                marks = mfma16(T{}, mark, one, marks);
-                            }
-#pragma unroll
-                            for (int i = 0; i < 16; ++i) o[eb][i] += odd_sum(marks[i]);
-                        }
 #pragma unroll
                         for (int x = 0; x < 2; ++x) o[eb] = mfma16(T{}, v[x], p[x], o[eb]);
                     }
+                    if (bad)
+#pragma unroll
+                        for (int i = 0; i < 16; ++i) seen |= (p[i / 8][i % 8] & 0x7fff) ? 1u << (8 * (i / 4) + i % 4) : 0u;
+                }
+                if (bad) {                                                // what an odd value does, to those that see it
+                    seen = other_half_or(seen << (4 * half));
+#pragma unroll
+                    for (int eb = 0; eb < EB; ++eb)
+#pragma unroll
+                        for (int i = 0; i < 16; ++i) {
+                            const int e = eb * 32 + 8 * (i / 4) + 4 * half + i % 4;
+                            const bool pos = infs[buf][0][b][e] & seen, neg = infs[buf][1][b][e] & seen;
+                            if (pos || neg) o[eb][i] += pos && neg ? __builtin_nanf("") : pos ? INFINITY : -INFINITY;
+                        }
                 }
             }
         }
-        if (tile >= 0) put(tile, buf ^ 1, turn & 3);                      // last read a turn ago, behind the barrier
+        if (tile >= 0) put(tile, buf ^ 1, turn);                      // last read a turn ago, behind the barrier
         __syncthreads();
     }
 
@@ -457,9 +474,11 @@ int launch(const krk_attention_args& a, const AttnTiles& g, void* scratch, hipSt
         ranges = r;
         hipLaunchKernelGGL(attn_ranges_kernel, dim3((unsigned)(((long)a.N * tiles + 3) / 4)), dim3(256), 0, s, a, r, tiles, g.keys);
     }
-    const long blocks = ((long)a.N * a.Hk + 7) / 8 * 8 * qblocks * (a.H / a.Hk);
+    const long groups = (long)a.N * a.Hk;
+    const int cut = groups % 8 == 0 ? 1 : groups % 4 == 0 ? 2 : groups % 2 == 0 ? 4 : 8;
+    const long blocks = groups * cut * ((qblocks * (long)(a.H / a.Hk) + cut - 1) / cut);
     if (blocks > 0x7fffff00L) return -4;
-    hipLaunchKernelGGL((attn_tile_kernel<T, EP, NW>), dim3((unsigned)blocks, g.splits), dim3(NW * 64), 0, s, a, qblocks, g.splits, tiles, ranges);
+    hipLaunchKernelGGL((attn_tile_kernel<T, EP, NW>), dim3((unsigned)blocks, g.splits), dim3(NW * 64), 0, s, a, qblocks, cut, g.splits, tiles, ranges);
     return hipGetLastError() == hipSuccess ? 0 : -1;
 }
 
