@@ -98,11 +98,16 @@ __global__ __launch_bounds__(256) void attn_ranges_kernel(krk_attention_args a, 
     if (lane == 0) out[id] = make_int2(lo, hi);
 }
 
+// a statement for every score of a lane: s[x][i]
+#define EACH(...)                          \
+    _Pragma("unroll") for (int x = 0; x < NJ; ++x) _Pragma("unroll") for (int i = 0; i < 16; ++i) { __VA_ARGS__; }
+
 template <class T, int EP, int NW>
-__global__ __launch_bounds__(NW * 64, EP * sizeof(T) > 256 ? 1 : sizeof(T) == 2 && EP <= 64 ? 3 : 2) void attn_tile_kernel(krk_attention_args a, int qblocks, int cut, int splits, int tiles, const int2* ranges) {
+__global__ __launch_bounds__(NW * 64, EP * sizeof(T) > 256 ? 1 : 2) void attn_tile_kernel(krk_attention_args a, int qblocks, int cut, int batch, int splits, int tiles, const int2* ranges) {
     using G = Geo<T, EP, NW>;
     constexpr bool F32 = G::F32;
     constexpr int BK = G::BK, SB = G::SB, EB = G::EB, KLD = G::KLD, VLD = G::VLD, CV = G::CV, NT = NW * 64;
+    constexpr int NJ = !F32 && NW == 4 && EP <= 64 ? 2 : 1;               // blocks of 32 keys at once: more to overlap, where the registers allow it
     constexpr int CPT = (G::CHUNKS + NT - 1) / NT, CPR = EP / CV;         // chunks per thread and per row
     __shared__ __attribute__((aligned(16))) T Kbuf[2][BK * KLD];
     __shared__ __attribute__((aligned(16))) T Vbuf[2][BK * VLD];
@@ -111,10 +116,13 @@ __global__ __launch_bounds__(NW * 64, EP * sizeof(T) > 256 ? 1 : sizeof(T) == 2 
     __shared__ unsigned infs[2][2][SB][EP];                               // where the tile's odd values were: +inf / -inf (NaN: both), a bit per key
 
     // All query blocks and heads that share a key head run on one XCD (workgroups go round the eight of them), so its L2 holds their keys; where
-    // the key heads do not go round evenly each is cut into `cut` interleaved parts.  The blocks with the longest causal rows come first.
+    // the key heads do not go round evenly each is cut into `cut` interleaved parts.  `batch` of them, as many as the L2 holds, are taken together,
+    // the blocks with the longest causal rows first, so that the short ones fill the end.
     const int rep = a.H / a.Hk, inner = qblocks * rep, part_size = (inner + cut - 1) / cut;
-    const long id = blockIdx.x / 8, group = (blockIdx.x & 7) + 8 * (id / part_size);
-    const int in = (int)(id % part_size) * cut + (int)(group % cut);
+    const long id = blockIdx.x / 8, per_xcd = gridDim.x / 8 / part_size, first = id / ((long)part_size * batch) * batch;
+    const int width = (int)min((long)batch, per_xcd - first), at = (int)(id - first * part_size);
+    const long group = (blockIdx.x & 7) + 8 * (first + at % width);
+    const int in = at / width * cut + (int)(group % cut);
     if (in >= inner) return;
     const long kvh = group / cut;
     const int n = kvh / a.Hk, hk = kvh % a.Hk;
@@ -297,64 +305,61 @@ __global__ __launch_bounds__(NW * 64, EP * sizeof(T) > 256 ? 1 : sizeof(T) == 2 
         }
         if (see) {
             const T *Ks = Kbuf[buf], *Vs = Vbuf[buf];
-#pragma unroll 1
-            for (int b = 0; b < SB; ++b) {
-                // S^T = K Q^T of 32 keys
-                f32x16 s;
 #pragma unroll
-                for (int i = 0; i < 16; ++i) s[i] = 0.f;
-                const T* kb = &Ks[(b * 32 + col) * KLD];
-                if constexpr (F32) {
+            for (int b0 = 0; b0 < SB; b0 += NJ) {
+                // S^T = K Q^T of NJ blocks of 32 keys; register i of block b: key k0 + 32 b + 8 (i / 4) + 4 half + i % 4
+                f32x16 s[NJ];
 #pragma unroll
-                    for (int g = 0; g < EP / 8; ++g) {
-                        const f32x4 k = *(const f32x4*)&kb[8 * g + 4 * half];
+                for (int x = 0; x < NJ; ++x) {
 #pragma unroll
-                        for (int i = 0; i < 4; ++i) s = __builtin_amdgcn_mfma_f32_32x32x2f32(k[i], q32[g][i], s, 0, 0, 0);
+                    for (int i = 0; i < 16; ++i) s[x][i] = 0.f;
+                    const T* kb = &Ks[((b0 + x) * 32 + col) * KLD];
+                    if constexpr (F32) {
+#pragma unroll
+                        for (int g = 0; g < EP / 8; ++g) {
+                            const f32x4 k = *(const f32x4*)&kb[8 * g + 4 * half];
+#pragma unroll
+                            for (int i = 0; i < 4; ++i) s[x] = __builtin_amdgcn_mfma_f32_32x32x2f32(k[i], q32[g][i], s[x], 0, 0, 0);
+                        }
+                    } else {
+#pragma unroll
+                        for (int ks = 0; ks < EP / 16; ++ks) s[x] = mfma16(T{}, *(const s16x8*)&kb[16 * ks + 8 * half], q16[ks], s[x]);
                     }
-                } else {
-#pragma unroll
-                    for (int ks = 0; ks < EP / 16; ++ks) s = mfma16(T{}, *(const s16x8*)&kb[16 * ks + 8 * half], q16[ks], s);
                 }
-                // register i: key k0 + 32 b + 8 (i / 4) + 4 half + i % 4
                 float scale = c;
                 if (!plain) {
                     scale = 1.f;
                     if (a.cap > 0.f) {
                         if constexpr (F32) {
                             const float raw = c * (1.f / LOG2E);
-#pragma unroll
-                            for (int i = 0; i < 16; ++i) s[i] = seq_cap<T>(s[i] * raw, a.cap, rcap) * LOG2E;
+                            EACH(s[x][i] = seq_cap<T>(s[x][i] * raw, a.cap, rcap) * LOG2E);
                         } else {                                          // cap tanh(x) = cap - 2 cap / (1 + e^2x): 2^-23 of cap off at most
                             const float cl = a.cap * LOG2E, cx = 2.f * c * rcap;
-#pragma unroll
-                            for (int i = 0; i < 16; ++i)
-                                s[i] = __builtin_fmaf(-2.f * cl, __builtin_amdgcn_rcpf(1.f + __builtin_amdgcn_exp2f(s[i] * cx)), cl);
+                            EACH(s[x][i] = __builtin_fmaf(-2.f * cl, __builtin_amdgcn_rcpf(1.f + __builtin_amdgcn_exp2f(s[x][i] * cx)), cl));
                         }
                     } else {
-#pragma unroll
-                        for (int i = 0; i < 16; ++i) s[i] *= c;
+                        EACH(s[x][i] *= c);
                     }
                     if (a.slopes) {
-                        const float d0 = (float)(mine.p - k0 - 32 * b - 4 * half);
-#pragma unroll
-                        for (int i = 0; i < 16; ++i) s[i] = __builtin_fmaf(-slope, fabsf(d0 - (float)(8 * (i / 4) + i % 4)), s[i]);
+                        const float d0 = (float)(mine.p - k0 - 32 * b0 - 4 * half);
+                        EACH(s[x][i] = __builtin_fmaf(-slope, fabsf(d0 - (float)(32 * x + 8 * (i / 4) + i % 4)), s[x][i]));
                     }
                 }
                 if (part) {
-                    const int room = lim - k0 - 32 * b - 4 * half;
+                    const int room = lim - k0 - 32 * b0 - 4 * half;
+                    EACH(s[x][i] = 32 * x + 8 * (i / 4) + i % 4 < room ? s[x][i] : -INFINITY);
+                    if (docs)
 #pragma unroll
-                    for (int i = 0; i < 16; ++i) s[i] = 8 * (i / 4) + i % 4 < room ? s[i] : -INFINITY;
-                    if (docs) {
-                        int4 ids[4];
+                        for (int x = 0; x < NJ; ++x) {
+                            int4 ids[4];
 #pragma unroll
-                        for (int g = 0; g < 4; ++g) ids[g] = *(const int4*)&dbuf[buf][32 * b + 8 * g + 4 * half];
+                            for (int g = 0; g < 4; ++g) ids[g] = *(const int4*)&dbuf[buf][32 * (b0 + x) + 8 * g + 4 * half];
 #pragma unroll
-                        for (int i = 0; i < 16; ++i) s[i] = (&ids[i / 4].x)[i % 4] == doc ? s[i] : -INFINITY;
-                    }
+                            for (int i = 0; i < 16; ++i) s[x][i] = (&ids[i / 4].x)[i % 4] == doc ? s[x][i] : -INFINITY;
+                        }
                 }
-                float top = s[0];
-#pragma unroll
-                for (int i = 1; i < 16; ++i) top = fmaxf(top, s[i]);
+                float top = s[0][0];
+                EACH(top = fmaxf(top, s[x][i]));
                 top = other_half_max(top) * scale;
                 // The reference point moves only when a score passes it by 2^8: weights up to 256 are as exact, and most tiles leave the sums alone.
                 if (__ballot(top > m + 8.f)) {
@@ -367,63 +372,56 @@ __global__ __launch_bounds__(NW * 64, EP * sizeof(T) > 256 ? 1 : sizeof(T) == 2 
                         for (int i = 0; i < 16; ++i) o[eb][i] *= f;
                 }
                 const float ref = m == -INFINITY ? 0.f : m;
-                float sum = 0.f;
-#pragma unroll
-                for (int i = 0; i < 16; ++i) {
-                    s[i] = __builtin_amdgcn_exp2f(__builtin_fmaf(s[i], scale, -ref));
-                    sum += s[i];
-                }
-                l += sum;
+                float sum[4] = {0.f, 0.f, 0.f, 0.f};
+                EACH(s[x][i] = __builtin_amdgcn_exp2f(__builtin_fmaf(s[x][i], scale, -ref)); sum[i % 4] += s[x][i]);
+                l += (sum[0] + sum[1]) + (sum[2] + sum[3]);
 
                 // O^T += V^T P^T
-                unsigned seen = 0;                                        // of this half's keys, those with a weight
+                unsigned seen[NJ];                                        // of this half's keys, those with a weight
                 if constexpr (F32) {
-#pragma unroll
-                    for (int eb = 0; eb < EB; ++eb) {
-                        const T* vb = &Vs[(b * 32 + 4 * half) * VLD + eb * 32 + col];
-#pragma unroll
-                        for (int i = 0; i < 16; ++i)
-                            o[eb] = __builtin_amdgcn_mfma_f32_32x32x2f32(vb[(8 * (i / 4) + i % 4) * VLD], s[i], o[eb], 0, 0, 0);
-                    }
-                    if (bad)
-#pragma unroll
-                        for (int i = 0; i < 16; ++i) seen |= s[i] != 0.f ? 1u << (8 * (i / 4) + i % 4) : 0u;
-                } else {
-                    s16x8 p[2];
-#pragma unroll
-                    for (int x = 0; x < 2; ++x)
-#pragma unroll
-                        for (int i = 0; i < 8; ++i) p[x][i] = __builtin_bit_cast(short, from_f<T>(s[8 * x + i]));
-                    // lane l gets, for channel l % 32, the four keys of its half: 16 lanes hold four rows of 16 channels, read transposed
-                    const T* vb = &Vs[(32 * b + 4 * half + (col & 15) / 4) * VLD + 16 * (col >> 4) + 4 * (col & 3)];
-#pragma unroll
-                    for (int eb = 0; eb < EB; ++eb) {
-                        s16x8 v[2];
-#pragma unroll
-                        for (int x = 0; x < 2; ++x) {
-                            typedef __attribute__((address_space(3))) s16x4 lds4;
-                            const s16x4 lo = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds4*)&vb[16 * x * VLD + eb * 32]);
-                            const s16x4 hi = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds4*)&vb[(16 * x + 8) * VLD + eb * 32]);
-                            v[x] = __builtin_shufflevector(lo, hi, 0, 1, 2, 3, 4, 5, 6, 7);
-                        }
-#pragma unroll
-                        for (int x = 0; x < 2; ++x) o[eb] = mfma16(T{}, v[x], p[x], o[eb]);
-                    }
-                    if (bad)
-#pragma unroll
-                        for (int i = 0; i < 16; ++i) seen |= (p[i / 8][i % 8] & 0x7fff) ? 1u << (8 * (i / 4) + i % 4) : 0u;
-                }
-                if (bad) {                                                // what an odd value does, to those that see it
-                    seen = other_half_or(seen << (4 * half));
 #pragma unroll
                     for (int eb = 0; eb < EB; ++eb)
 #pragma unroll
-                        for (int i = 0; i < 16; ++i) {
-                            const int e = eb * 32 + 8 * (i / 4) + 4 * half + i % 4;
-                            const bool pos = infs[buf][0][b][e] & seen, neg = infs[buf][1][b][e] & seen;
-                            if (pos || neg) o[eb][i] += pos && neg ? __builtin_nanf("") : pos ? INFINITY : -INFINITY;
+                        for (int x = 0; x < NJ; ++x) {
+                            const T* vb = &Vs[((b0 + x) * 32 + 4 * half) * VLD + eb * 32 + col];
+#pragma unroll
+                            for (int i = 0; i < 16; ++i)
+                                o[eb] = __builtin_amdgcn_mfma_f32_32x32x2f32(vb[(8 * (i / 4) + i % 4) * VLD], s[x][i], o[eb], 0, 0, 0);
                         }
+                    if (bad) {
+                        EACH(seen[x] = (i ? seen[x] : 0u) | (s[x][i] != 0.f ? 1u << (8 * (i / 4) + i % 4) : 0u));
+                    }
+                } else {
+                    s16x8 p[2 * NJ];
+                    EACH(p[2 * x + i / 8][i % 8] = __builtin_bit_cast(short, from_f<T>(s[x][i])));
+                    // lane l gets, for channel l % 32, the four keys of its half: 16 lanes hold four rows of 16 channels, read transposed
+                    const T* vb = &Vs[(32 * b0 + 4 * half + (col & 15) / 4) * VLD + 16 * (col >> 4) + 4 * (col & 3)];
+#pragma unroll
+                    for (int eb = 0; eb < EB; ++eb)
+#pragma unroll
+                        for (int x = 0; x < 2 * NJ; ++x) {
+                            typedef __attribute__((address_space(3))) s16x4 lds4;
+                            const s16x4 lo = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds4*)&vb[16 * x * VLD + eb * 32]);
+                            const s16x4 hi = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds4*)&vb[(16 * x + 8) * VLD + eb * 32]);
+                            o[eb] = mfma16(T{}, __builtin_shufflevector(lo, hi, 0, 1, 2, 3, 4, 5, 6, 7), p[x], o[eb]);
+                        }
+                    if (bad) {
+                        EACH(seen[x] = (i ? seen[x] : 0u) | ((p[2 * x + i / 8][i % 8] & 0x7fff) ? 1u << (8 * (i / 4) + i % 4) : 0u));
+                    }
                 }
+                if (bad)                                                  // what an odd value does, to those that see it
+#pragma unroll
+                    for (int x = 0; x < NJ; ++x) {
+                        const unsigned see = other_half_or(seen[x] << (4 * half));
+#pragma unroll
+                        for (int eb = 0; eb < EB; ++eb)
+#pragma unroll
+                            for (int i = 0; i < 16; ++i) {
+                                const int e = eb * 32 + 8 * (i / 4) + 4 * half + i % 4;
+                                const bool pos = infs[buf][0][b0 + x][e] & see, neg = infs[buf][1][b0 + x][e] & see;
+                                if (pos || neg) o[eb][i] += pos && neg ? __builtin_nanf("") : pos ? INFINITY : -INFINITY;
+                            }
+                    }
             }
         }
         if (tile >= 0) put(tile, buf ^ 1, turn);                      // last read a turn ago, behind the barrier
@@ -476,9 +474,11 @@ int launch(const krk_attention_args& a, const AttnTiles& g, void* scratch, hipSt
     }
     const long groups = (long)a.N * a.Hk;
     const int cut = groups % 8 == 0 ? 1 : groups % 4 == 0 ? 2 : groups % 2 == 0 ? 4 : 8;
+    // only causal rows differ in length by their place; elsewhere one key head at a time is better for the L2 (lines: 138 against 143 us)
+    const int batch = !a.causal || a.documents ? 1 : (int)max(1L, min(64L, (4L << 20) / (2L * a.Tk * a.E * (long)sizeof(T) / cut + 1)));
     const long blocks = groups * cut * ((qblocks * (long)(a.H / a.Hk) + cut - 1) / cut);
     if (blocks > 0x7fffff00L) return -4;
-    hipLaunchKernelGGL((attn_tile_kernel<T, EP, NW>), dim3((unsigned)blocks, g.splits), dim3(NW * 64), 0, s, a, qblocks, cut, g.splits, tiles, ranges);
+    hipLaunchKernelGGL((attn_tile_kernel<T, EP, NW>), dim3((unsigned)blocks, g.splits), dim3(NW * 64), 0, s, a, qblocks, cut, batch, g.splits, tiles, ranges);
     return hipGetLastError() == hipSuccess ? 0 : -1;
 }
 

@@ -2,68 +2,248 @@
 //
 //   h_i = exp(s_i A) h_{i-1} + s_i x_i B_i,   y_i = C_i . h_i + skip x_i   (times z sigmoid(z)),   s_i = softplus(dt_i + bias)
 //
-// LP lanes share a channel, SL states each, in registers for the whole row.
+// Per channel, step and state: an exponential, two products and two multiply-adds; per channel and step 6 to 16 bytes.  At 16 states the vector
+// units bound it, not memory.  A lane owns a channel (LP lanes share one with more than SL states) and keeps its states and rates in
+// registers for a whole row; lanes lie along the channels, so every access of a step is contiguous.  B and C, the same for all channels of a
+// group, go through LDS as fp32, U steps at a time; the next U steps' inputs are in flight while U steps are computed.
+//
+// Few rows do not fill the chip with channels alone: then the time axis is cut into chunks.  One pass gives every chunk's end state from a
+// zero start and the sum of its steps -- the decay over a chunk is exp(A sum) --, a second joins the chunks in order, and the main pass starts every
+// chunk from its true state.  That costs four fifths of the work again, so it is done only where half of the chip would idle.
 #include "seq.h"
 
 namespace {
 
 constexpr float LOG2E = 1.4426950408889634f;
+constexpr int U = 8;
 
-template <class T, int LP, int SL>
-__global__ __launch_bounds__(256) void scan_seq_kernel(krk_scan_args a) {
-    const int id = blockIdx.x * 256 + threadIdx.x;
-    const int d = id / LP, part = id % LP;
-    const bool live = d < a.D;
-    const int dd = live ? d : 0, s0 = part * SL, g = dd / (a.D / a.G);
+struct ScanCut {
+    int chunks, len;       // time chunks and steps of each
+    float* part;           // [N][chunks - 1][D][S]: end states from a zero start, after the join the states in front of the next chunk
+    float* sums;           // [N][chunks - 1][D]: sums of the steps
+};
+
+template <class T, int LP, int SL, bool MAIN>
+__global__ __launch_bounds__(256) void scan_seq_kernel(krk_scan_args a, ScanCut cut) {
+    constexpr int SP = LP * SL, NBC = (U * SP + 255) / 256;      // values of B (and of C) that a thread stages per U steps
+    __shared__ __attribute__((aligned(16))) float Bs[2][U][SP], Cs[MAIN ? 2 : 1][MAIN ? U : 1][SP];
+    const int per = a.D / a.G, per_block = 256 / LP, blocks_g = (per + per_block - 1) / per_block;
+    const int g = blockIdx.x / blocks_g, dg = (blockIdx.x - g * blocks_g) * per_block + threadIdx.x / LP, part = threadIdx.x % LP;
+    const bool live = dg < per;
+    const unsigned d = g * per + (live ? dg : 0);
+    const int s0 = part * SL, chunk = blockIdx.y;
     float A[SL];
 #pragma unroll
-    for (int j = 0; j < SL; ++j) A[j] = s0 + j < a.S ? a.A[(long)dd * a.S + s0 + j] * LOG2E : 0.f;
-    const float bias = a.dt_bias ? a.dt_bias[dd] : 0.f, skip = a.skip ? a.skip[dd] : 0.f;
-    for (int n = blockIdx.y; n < a.N; n += gridDim.y) {
-        const int len = seq_len(a.lens, n, a.T);
-        float h[SL];
+    for (int j = 0; j < SL; ++j) A[j] = s0 + j < a.S ? a.A[(long)d * a.S + s0 + j] * LOG2E : 0.f;
+    const float bias = a.dt_bias ? a.dt_bias[d] : 0.f, skip = a.skip ? a.skip[d] : 0.f;
+    for (int n = blockIdx.z; n < a.N; n += gridDim.z) {
+        const int len = __builtin_amdgcn_readfirstlane(seq_len(a.lens, n, a.T));
+        const int i0 = chunk * cut.len, i1 = min(i0 + cut.len, len);
+        const T *xp = (const T*)a.x + n * a.x_n, *dp = (const T*)a.dt + n * a.dt_n, *zp = a.z ? (const T*)a.z + n * a.z_n : nullptr;
+        const T *bp = (const T*)a.B + n * a.b_n + (long)g * a.S, *cp = (const T*)a.C + n * a.c_n + (long)g * a.S;
+        T* yp = (T*)a.y + n * a.y_n;
+        float h[SL], sum = 0.f;
 #pragma unroll
-        for (int j = 0; j < SL; ++j) h[j] = a.state && s0 + j < a.S ? a.state[n * a.state_n + (long)dd * a.S + s0 + j] : 0.f;
-        for (int i = 0; i < len; ++i) {
-            const long t = a.reverse ? len - 1 - i : i;
-            const float x = to_f(((const T*)a.x)[n * a.x_n + t * a.x_t + dd]);
-            float s = to_f(((const T*)a.dt)[n * a.dt_n + t * a.dt_t + dd]) + bias;
-            if (a.softplus) s = seq_softplus(s);
-            const T* B = (const T*)a.B + n * a.b_n + t * a.b_t + (long)g * a.S + s0;
-            const T* C = (const T*)a.C + n * a.c_n + t * a.c_t + (long)g * a.S + s0;
-            const float sx = s * x;
-            float y = 0.f;
+        for (int j = 0; j < SL; ++j) {
+            h[j] = 0.f;
+            if (MAIN && s0 + j < a.S) {
+                if (chunk > 0) h[j] = cut.part[(((long)n * (cut.chunks - 1) + chunk - 1) * a.D + d) * a.S + s0 + j];
+                else if (a.state) h[j] = a.state[n * a.state_n + (long)d * a.S + s0 + j];
+            }
+        }
+        T xr[U], dr[U], zr[U], br[NBC], cr[NBC];
+        auto step = [&](int i) -> long { i = min(i, i1 - 1); return a.reverse ? len - 1 - i : i; };
+        auto fetch = [&](int i) {                                 // steps behind the end repeat the last one; they are not computed
 #pragma unroll
-            for (int j = 0; j < SL; ++j) {
-                const bool in = s0 + j < a.S;
-                h[j] = __builtin_fmaf(__builtin_amdgcn_exp2f(s * A[j]), h[j], sx * (in ? to_f(B[j]) : 0.f));
-                y = __builtin_fmaf(in ? to_f(C[j]) : 0.f, h[j], y);
+            for (int u = 0; u < U; ++u) {
+                const long t = step(i + u);
+                xr[u] = (xp + t * a.x_t)[d];
+                dr[u] = (dp + t * a.dt_t)[d];
+                if (MAIN && zp) zr[u] = (zp + t * a.z_t)[d];
             }
 #pragma unroll
-            for (int m = 1; m < LP; m <<= 1) y += __shfl_xor(y, m);
-            y = __builtin_fmaf(skip, x, y);
-            if (a.z) y *= seq_silu(to_f(((const T*)a.z)[n * a.z_n + t * a.z_t + dd]));
-            if (live && part == 0) ((T*)a.y)[n * a.y_n + t * a.y_t + dd] = from_f<T>(y);
+            for (int k = 0; k < NBC; ++k) {
+                const int id = threadIdx.x + 256 * k, u = min(id / SP, U - 1), j = min(id % SP, a.S - 1);
+                const long t = step(i + u);
+                br[k] = bp[t * a.b_t + j];
+                if (MAIN) cr[k] = cp[t * a.c_t + j];
+            }
+        };
+        auto put = [&](int buf) {                                 // states that do not exist get B = C = 0
+#pragma unroll
+            for (int k = 0; k < NBC; ++k) {
+                const int id = threadIdx.x + 256 * k;
+                if (U * SP % 256 == 0 || id < U * SP) {
+                    (&Bs[buf][0][0])[id] = id % SP < a.S ? to_f(br[k]) : 0.f;
+                    if (MAIN) (&Cs[buf][0][0])[id] = id % SP < a.S ? to_f(cr[k]) : 0.f;
+                }
+            }
+        };
+        if (i0 < i1) {
+            fetch(i0);
+            put(0);
         }
-        if (live && part == 0)
-            for (int t = len; t < a.T; ++t) ((T*)a.y)[n * a.y_n + (long)t * a.y_t + dd] = from_f<T>(0.f);
-        if (live && a.state_out)
+        __syncthreads();
+        int buf = 0;
+        for (int i = i0; i < i1; i += U, buf ^= 1) {
+            T xc[U], dc[U], zc[U];
+#pragma unroll
+            for (int u = 0; u < U; ++u) xc[u] = xr[u], dc[u] = dr[u], zc[u] = zr[u];
+            const bool more = i + U < i1;
+            if (more) fetch(i + U);
+#pragma unroll
+            for (int u = 0; u < U; ++u) {
+                if (i + u >= i1) break;
+                const float x = to_f(xc[u]);
+                float s = to_f(dc[u]) + bias;
+                if (a.softplus) s = seq_softplus(s);
+                const float sx = s * x;
+                float y0 = 0.f, y1 = 0.f;
+                if (!MAIN) sum += s;
+#pragma unroll
+                for (int j = 0; j < SL; j += 4) {
+                    const f32x4 b = *(const f32x4*)&Bs[buf][u][s0 + j];
+                    f32x4 c = {0.f, 0.f, 0.f, 0.f};
+                    if (MAIN) c = *(const f32x4*)&Cs[MAIN ? buf : 0][MAIN ? u : 0][s0 + j];
+#pragma unroll
+                    for (int v = 0; v < 4; ++v) {
+                        h[j + v] = __builtin_fmaf(__builtin_amdgcn_exp2f(s * A[j + v]), h[j + v], sx * b[v]);
+                        if (MAIN) (v & 1 ? y1 : y0) = __builtin_fmaf(c[v], h[j + v], v & 1 ? y1 : y0);
+                    }
+                }
+                if (MAIN) {
+                    float y = y0 + y1;
+#pragma unroll
+                    for (int m = 1; m < LP; m <<= 1) y += __shfl_xor(y, m);
+                    y = __builtin_fmaf(skip, x, y);
+                    if (zp) y *= seq_silu(to_f(zc[u]));
+                    const long t = a.reverse ? len - 1 - (i + u) : i + u;
+                    if (live && part == 0) (yp + t * a.y_t)[d] = from_f<T>(y);
+                }
+            }
+            if (more) put(buf ^ 1);
+            __syncthreads();
+        }
+        if (!live) continue;
+        if (MAIN) {
+            if (part == 0)
+                for (int t = max(i0, len); t < min(i0 + cut.len, a.T); ++t) (yp + (long)t * a.y_t)[d] = from_f<T>(0.f);
+            if (a.state_out && chunk == max(len - 1, 0) / cut.len)
+#pragma unroll
+                for (int j = 0; j < SL; ++j)
+                    if (s0 + j < a.S) a.state_out[n * a.out_n + (long)d * a.S + s0 + j] = h[j];
+        } else {
+            const long at = ((long)n * (cut.chunks - 1) + chunk) * a.D + d;
 #pragma unroll
             for (int j = 0; j < SL; ++j)
-                if (s0 + j < a.S) a.state_out[n * a.out_n + (long)dd * a.S + s0 + j] = h[j];
+                if (s0 + j < a.S) cut.part[at * a.S + s0 + j] = h[j];
+            if (part == 0) cut.sums[at] = sum;
+        }
     }
+}
+
+// the states in front of every chunk: one lane per (channel, state), the chunks in order
+__global__ __launch_bounds__(256) void scan_join_kernel(krk_scan_args a, ScanCut cut) {
+    const long id = (long)blockIdx.x * 256 + threadIdx.x, ds = (long)a.D * a.S;
+    if (id >= ds) return;
+    const long d = id / a.S;
+    const float A = a.A[id] * LOG2E;
+    for (int n = blockIdx.y; n < a.N; n += gridDim.y) {
+        float h = a.state ? a.state[n * a.state_n + id] : 0.f;
+        float* p = cut.part + (long)n * (cut.chunks - 1) * ds + id;
+        const float* s = cut.sums + (long)n * (cut.chunks - 1) * a.D + d;
+#pragma unroll 8
+        for (int c = 0; c < cut.chunks - 1; ++c) {
+            h = __builtin_fmaf(__builtin_amdgcn_exp2f(s[(long)c * a.D] * A), h, p[c * ds]);
+            p[c * ds] = h;
+        }
+    }
+}
+
+// One step of every row: four states per lane, LP lanes per channel, so that the states are read and written by whole lines; bound by them.
+template <class T, int LP>
+__global__ __launch_bounds__(256) void scan_step_kernel(krk_scan_args a) {
+    const long id = (long)blockIdx.x * 256 + threadIdx.x;
+    const int part = id % LP, s0 = part * 4, nv = min(4, a.S - s0);
+    long row = id / LP;
+    const bool live = row < (long)a.N * a.D;
+    if (!live) row = 0;
+    const int n = row / a.D, d = row - (long)n * a.D, g = d / (a.D / a.G);
+    const bool on = seq_len(a.lens, n, 1) > 0;
+    const float x = to_f(((const T*)a.x)[n * a.x_n + d]);
+    float s = to_f(((const T*)a.dt)[n * a.dt_n + d]) + (a.dt_bias ? a.dt_bias[d] : 0.f);
+    float A[4], b[4], c[4], h[4] = {0.f, 0.f, 0.f, 0.f};
+    load_vec<float, 4>(a.A + (long)d * a.S + s0, nv, A);
+    load_vec<T, 4>((const T*)a.B + n * a.b_n + (long)g * a.S + s0, nv, b);
+    load_vec<T, 4>((const T*)a.C + n * a.c_n + (long)g * a.S + s0, nv, c);
+    if (a.state) load_vec<float, 4>(a.state + n * a.state_n + (long)d * a.S + s0, nv, h);
+    if (a.softplus) s = seq_softplus(s);
+    float y = 0.f;
+    if (on) {
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+            h[j] = __builtin_fmaf(__builtin_amdgcn_exp2f(s * A[j] * LOG2E), h[j], s * x * b[j]);
+            y = __builtin_fmaf(c[j], h[j], y);
+        }
+    }
+#pragma unroll
+    for (int m = 1; m < LP; m <<= 1) y += __shfl_xor(y, m);
+    if (!live) return;
+    if (a.state_out) store_vec<float, 4>(a.state_out + n * a.out_n + (long)d * a.S + s0, nv, h);
+    if (part) return;
+    y = __builtin_fmaf(a.skip ? a.skip[d] : 0.f, x, y);
+    if (a.z) y *= seq_silu(to_f(((const T*)a.z)[n * a.z_n + d]));
+    ((T*)a.y)[n * a.y_n + d] = from_f<T>(on ? y : 0.f);
+}
+
+int lanes_of(int S) { return S <= 16 ? 1 : S <= 64 ? 4 : 16; }
+
+// Chunks of the time axis: none while the channels give one wave per SIMD or the rows are short; else enough for four waves each, 64 steps at least.
+void cut_time(const krk_scan_args& a, ScanCut& c) {
+    const long waves = (long)a.N * a.D * lanes_of(a.S) / 64 + 1;
+    long chunks = waves > 768 ? 1 : min((long)a.T / 64, 4096 / waves);
+    chunks = max(1L, min(chunks, 1024L));
+    c.len = a.T > 0 ? (int)((a.T + chunks - 1) / chunks) : 1;
+    c.chunks = a.T > 0 ? (a.T + c.len - 1) / c.len : 1;
 }
 
 template <class T, int LP, int SL>
 int launch(const krk_scan_args& a, hipStream_t s) {
-    const long blocks = ((long)a.D * LP + 255) / 256;
-    if ((long)a.D * LP > 0x7fffff00L) return -4;
-    hipLaunchKernelGGL((scan_seq_kernel<T, LP, SL>), dim3((unsigned)blocks, (unsigned)min(a.N, 65535)), dim3(256), 0, s, a);
+    ScanCut c;
+    cut_time(a, c);
+    const long states = (long)a.N * (c.chunks - 1) * a.D;
+    c.part = (float*)a.workspace;
+    c.sums = c.part + states * a.S;
+    const int per_block = 256 / LP;
+    const long blocks = (long)a.G * ((a.D / a.G + per_block - 1) / per_block);
+    const unsigned rows = (unsigned)min(a.N, 65535);
+    if (blocks > 0x7fffff00L) return -4;
+    if (c.chunks > 1) {
+        hipLaunchKernelGGL((scan_seq_kernel<T, LP, SL, false>), dim3((unsigned)blocks, c.chunks - 1, rows), dim3(256), 0, s, a, c);
+        hipLaunchKernelGGL(scan_join_kernel, dim3((unsigned)(((long)a.D * a.S + 255) / 256), rows), dim3(256), 0, s, a, c);
+    }
+    hipLaunchKernelGGL((scan_seq_kernel<T, LP, SL, true>), dim3((unsigned)blocks, c.chunks, rows), dim3(256), 0, s, a, c);
+    return hipGetLastError() == hipSuccess ? 0 : -1;
+}
+
+template <class T, int LP>
+int launch_step(const krk_scan_args& a, hipStream_t s) {
+    const long blocks = ((long)a.N * a.D * LP + 255) / 256;
+    if (blocks > 0x7fffff00L) return -4;
+    hipLaunchKernelGGL((scan_step_kernel<T, LP>), dim3((unsigned)blocks), dim3(256), 0, s, a);
     return hipGetLastError() == hipSuccess ? 0 : -1;
 }
 
 template <class T>
 int by_states(const krk_scan_args& a, hipStream_t s) {
+    if (a.T == 1) {
+        if (a.S <= 4) return launch_step<T, 1>(a, s);
+        if (a.S <= 8) return launch_step<T, 2>(a, s);
+        if (a.S <= 16) return launch_step<T, 4>(a, s);
+        if (a.S <= 64) return launch_step<T, 16>(a, s);
+        return launch_step<T, 64>(a, s);
+    }
+    if (a.S <= 8) return launch<T, 1, 8>(a, s);
     if (a.S <= 16) return launch<T, 1, 16>(a, s);
     if (a.S <= 64) return launch<T, 4, 16>(a, s);
     return launch<T, 16, 16>(a, s);
@@ -71,7 +251,11 @@ int by_states(const krk_scan_args& a, hipStream_t s) {
 
 }  // namespace
 
-long krk_scan_workspace(const krk_scan_args&) { return 0; }
+long krk_scan_workspace(const krk_scan_args& a) {
+    ScanCut c;
+    cut_time(a, c);
+    return c.chunks > 1 ? (long)a.N * (c.chunks - 1) * a.D * (a.S + 1) * (long)sizeof(float) : 0;
+}
 
 int krk_launch_selective_scan(const krk_scan_args& a, hipStream_t s) {
     return a.type == KRK_TYPE_F32 ? by_states<float>(a, s) : a.type == KRK_TYPE_BF16 ? by_states<bf16_t>(a, s) : by_states<f16_t>(a, s);
