@@ -23,6 +23,16 @@ struct ScanCut {
     float* sums;           // [N][chunks - 1][D]: sums of the steps
 };
 
+// SL states of a lane, four at a time; zeros where there are none
+template <int SL> __device__ __forceinline__ void load_states(const float* p, int n, float (&v)[SL]) {
+#pragma unroll
+    for (int j = 0; j < SL; j += 4) load_vec<float, 4>(p + j, n - j, *reinterpret_cast<float (*)[4]>(&v[j]));
+}
+template <int SL> __device__ __forceinline__ void store_states(float* p, int n, const float (&v)[SL]) {
+#pragma unroll
+    for (int j = 0; j < SL; j += 4) store_vec<float, 4>(p + j, n - j, *reinterpret_cast<const float (*)[4]>(&v[j]));
+}
+
 template <class T, int LP, int SL, bool MAIN>
 __global__ __launch_bounds__(256) void scan_seq_kernel(krk_scan_args a, ScanCut cut) {
     constexpr int SP = LP * SL, NBC = (U * SP + 255) / 256;      // values of B (and of C) that a thread stages per U steps
@@ -33,8 +43,9 @@ __global__ __launch_bounds__(256) void scan_seq_kernel(krk_scan_args a, ScanCut 
     const unsigned d = g * per + (live ? dg : 0);
     const int s0 = part * SL, chunk = blockIdx.y;
     float A[SL];
+    load_states(a.A + (long)d * a.S + s0, a.S - s0, A);
 #pragma unroll
-    for (int j = 0; j < SL; ++j) A[j] = s0 + j < a.S ? a.A[(long)d * a.S + s0 + j] * LOG2E : 0.f;
+    for (int j = 0; j < SL; ++j) A[j] *= LOG2E;
     const float bias = a.dt_bias ? a.dt_bias[d] : 0.f, skip = a.skip ? a.skip[d] : 0.f;
     for (int n = blockIdx.z; n < a.N; n += gridDim.z) {
         const int len = __builtin_amdgcn_readfirstlane(seq_len(a.lens, n, a.T));
@@ -44,13 +55,9 @@ __global__ __launch_bounds__(256) void scan_seq_kernel(krk_scan_args a, ScanCut 
         T* yp = (T*)a.y + n * a.y_n;
         float h[SL], sum = 0.f;
 #pragma unroll
-        for (int j = 0; j < SL; ++j) {
-            h[j] = 0.f;
-            if (MAIN && s0 + j < a.S) {
-                if (chunk > 0) h[j] = cut.part[(((long)n * (cut.chunks - 1) + chunk - 1) * a.D + d) * a.S + s0 + j];
-                else if (a.state) h[j] = a.state[n * a.state_n + (long)d * a.S + s0 + j];
-            }
-        }
+        for (int j = 0; j < SL; ++j) h[j] = 0.f;
+        if (MAIN && chunk > 0) load_states(cut.part + (((long)n * (cut.chunks - 1) + chunk - 1) * a.D + d) * a.S + s0, a.S - s0, h);
+        else if (MAIN && a.state) load_states(a.state + n * a.state_n + (long)d * a.S + s0, a.S - s0, h);
         T xr[U], dr[U], zr[U], br[NBC], cr[NBC];
         auto step = [&](int i) -> long { i = min(i, i1 - 1); return a.reverse ? len - 1 - i : i; };
         auto fetch = [&](int i) {                                 // steps behind the end repeat the last one; they are not computed
@@ -69,37 +76,43 @@ __global__ __launch_bounds__(256) void scan_seq_kernel(krk_scan_args a, ScanCut 
                 if (MAIN) cr[k] = cp[t * a.c_t + j];
             }
         };
-        auto put = [&](int buf) {                                 // states that do not exist get B = C = 0
+        auto put = [&](int i, int buf) {                          // states that do not exist and steps behind the end get B = C = 0
 #pragma unroll
             for (int k = 0; k < NBC; ++k) {
                 const int id = threadIdx.x + 256 * k;
+                const bool is = id % SP < a.S && i + id / SP < i1;
                 if (U * SP % 256 == 0 || id < U * SP) {
-                    (&Bs[buf][0][0])[id] = id % SP < a.S ? to_f(br[k]) : 0.f;
-                    if (MAIN) (&Cs[buf][0][0])[id] = id % SP < a.S ? to_f(cr[k]) : 0.f;
+                    (&Bs[buf][0][0])[id] = is ? to_f(br[k]) : 0.f;
+                    if (MAIN) (&Cs[buf][0][0])[id] = is ? to_f(cr[k]) : 0.f;
                 }
             }
         };
         if (i0 < i1) {
             fetch(i0);
-            put(0);
+            put(i0, 0);
         }
         __syncthreads();
         int buf = 0;
         for (int i = i0; i < i1; i += U, buf ^= 1) {
-            T xc[U], dc[U], zc[U];
+            // One stretch of code for U steps, so that their LDS reads and exponentials overlap: a step behind the end has s = x = B = C = 0,
+            // which leaves the states as they are.
+            float x[U], w[U], y[U];
+            T zc[U];
+            const int left = i1 - i;
 #pragma unroll
-            for (int u = 0; u < U; ++u) xc[u] = xr[u], dc[u] = dr[u], zc[u] = zr[u];
-            const bool more = i + U < i1;
-            if (more) fetch(i + U);
+            for (int u = 0; u < U; ++u) x[u] = to_f(xr[u]), w[u] = to_f(dr[u]) + bias, zc[u] = zr[u];
+            if (left > U) fetch(i + U);
+            if (a.softplus)
+#pragma unroll
+                for (int u = 0; u < U; ++u) w[u] = seq_softplus(w[u]);
+            if (left < U)
+#pragma unroll
+                for (int u = 0; u < U; ++u) x[u] = u < left ? x[u] : 0.f, w[u] = u < left ? w[u] : 0.f;
 #pragma unroll
             for (int u = 0; u < U; ++u) {
-                if (i + u >= i1) break;
-                const float x = to_f(xc[u]);
-                float s = to_f(dc[u]) + bias;
-                if (a.softplus) s = seq_softplus(s);
-                const float sx = s * x;
+                const float wx = w[u] * x[u];
                 float y0 = 0.f, y1 = 0.f;
-                if (!MAIN) sum += s;
+                if (!MAIN) sum += w[u];
 #pragma unroll
                 for (int j = 0; j < SL; j += 4) {
                     const f32x4 b = *(const f32x4*)&Bs[buf][u][s0 + j];
@@ -107,36 +120,37 @@ __global__ __launch_bounds__(256) void scan_seq_kernel(krk_scan_args a, ScanCut 
                     if (MAIN) c = *(const f32x4*)&Cs[MAIN ? buf : 0][MAIN ? u : 0][s0 + j];
 #pragma unroll
                     for (int v = 0; v < 4; ++v) {
-                        h[j + v] = __builtin_fmaf(__builtin_amdgcn_exp2f(s * A[j + v]), h[j + v], sx * b[v]);
+                        h[j + v] = __builtin_fmaf(__builtin_amdgcn_exp2f(w[u] * A[j + v]), h[j + v], wx * b[v]);
                         if (MAIN) (v & 1 ? y1 : y0) = __builtin_fmaf(c[v], h[j + v], v & 1 ? y1 : y0);
                     }
                 }
                 if (MAIN) {
-                    float y = y0 + y1;
+                    y[u] = y0 + y1;
 #pragma unroll
-                    for (int m = 1; m < LP; m <<= 1) y += __shfl_xor(y, m);
-                    y = __builtin_fmaf(skip, x, y);
-                    if (zp) y *= seq_silu(to_f(zc[u]));
-                    const long t = a.reverse ? len - 1 - (i + u) : i + u;
-                    if (live && part == 0) (yp + t * a.y_t)[d] = from_f<T>(y);
+                    for (int m = 1; m < LP; m <<= 1) y[u] += __shfl_xor(y[u], m);
+                    y[u] = __builtin_fmaf(skip, x[u], y[u]);
                 }
             }
-            if (more) put(buf ^ 1);
+            if (MAIN) {
+                if (zp)
+#pragma unroll
+                    for (int u = 0; u < U; ++u) y[u] *= seq_silu(to_f(zc[u]));
+                if (live && part == 0)
+#pragma unroll
+                    for (int u = 0; u < U; ++u)
+                        if (u < left) (yp + (long)(a.reverse ? len - 1 - (i + u) : i + u) * a.y_t)[d] = from_f<T>(y[u]);
+            }
+            if (left > U) put(i + U, buf ^ 1);
             __syncthreads();
         }
         if (!live) continue;
         if (MAIN) {
             if (part == 0)
                 for (int t = max(i0, len); t < min(i0 + cut.len, a.T); ++t) (yp + (long)t * a.y_t)[d] = from_f<T>(0.f);
-            if (a.state_out && chunk == max(len - 1, 0) / cut.len)
-#pragma unroll
-                for (int j = 0; j < SL; ++j)
-                    if (s0 + j < a.S) a.state_out[n * a.out_n + (long)d * a.S + s0 + j] = h[j];
+            if (a.state_out && chunk == max(len - 1, 0) / cut.len) store_states(a.state_out + n * a.out_n + (long)d * a.S + s0, a.S - s0, h);
         } else {
             const long at = ((long)n * (cut.chunks - 1) + chunk) * a.D + d;
-#pragma unroll
-            for (int j = 0; j < SL; ++j)
-                if (s0 + j < a.S) cut.part[at * a.S + s0 + j] = h[j];
+            store_states(cut.part + at * a.S + s0, a.S - s0, h);
             if (part == 0) cut.sums[at] = sum;
         }
     }
@@ -152,10 +166,21 @@ __global__ __launch_bounds__(256) void scan_join_kernel(krk_scan_args a, ScanCut
         float h = a.state ? a.state[n * a.state_n + id] : 0.f;
         float* p = cut.part + (long)n * (cut.chunks - 1) * ds + id;
         const float* s = cut.sums + (long)n * (cut.chunks - 1) * a.D + d;
-#pragma unroll 8
-        for (int c = 0; c < cut.chunks - 1; ++c) {
-            h = __builtin_fmaf(__builtin_amdgcn_exp2f(s[(long)c * a.D] * A), h, p[c * ds]);
-            p[c * ds] = h;
+        constexpr int B = 16;                                     // loads in flight: the chain itself is a multiply-add a chunk
+        for (int c0 = 0; c0 < cut.chunks - 1; c0 += B) {
+            float e[B], q[B];
+#pragma unroll
+            for (int c = 0; c < B; ++c) {
+                const long at = min(c0 + c, cut.chunks - 2);
+                e[c] = s[at * a.D];
+                q[c] = p[at * ds];
+            }
+#pragma unroll
+            for (int c = 0; c < B; ++c)
+                if (c0 + c < cut.chunks - 1) {
+                    h = __builtin_fmaf(__builtin_amdgcn_exp2f(e[c] * A), h, q[c]);
+                    p[(c0 + c) * ds] = h;
+                }
         }
     }
 }
@@ -198,10 +223,10 @@ __global__ __launch_bounds__(256) void scan_step_kernel(krk_scan_args a) {
 
 int lanes_of(int S) { return S <= 16 ? 1 : S <= 64 ? 4 : 16; }
 
-// Chunks of the time axis: none while the channels give one wave per SIMD or the rows are short; else enough for four waves each, 64 steps at least.
+// Chunks of the time axis: none while the channels give one wave per SIMD or the rows are short; else enough for two waves each, 64 steps at least.
 void cut_time(const krk_scan_args& a, ScanCut& c) {
     const long waves = (long)a.N * a.D * lanes_of(a.S) / 64 + 1;
-    long chunks = waves > 768 ? 1 : min((long)a.T / 64, 4096 / waves);
+    long chunks = waves > 768 ? 1 : min((long)a.T / 64, 2048 / waves);
     chunks = max(1L, min(chunks, 1024L));
     c.len = a.T > 0 ? (int)((a.T + chunks - 1) / chunks) : 1;
     c.chunks = a.T > 0 ? (a.T + c.len - 1) / c.len : 1;
