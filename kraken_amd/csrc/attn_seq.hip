@@ -10,6 +10,28 @@
 
 namespace {
 
+template <int CTRL> __device__ __forceinline__ float dpp(float v) {
+    return __builtin_bit_cast(float, __builtin_amdgcn_update_dpp(0, __builtin_bit_cast(int, v), CTRL, 0xf, 0xf, true));
+}
+// the sum over LE neighbouring lanes, in all of them: exchanges inside the vector registers (quads, half rows, rows, pairs of rows, halves)
+template <int LE> __device__ __forceinline__ float group_sum(float v) {
+    v += dpp<0xB1>(v);                                             // quad_perm 1 0 3 2
+    v += dpp<0x4E>(v);                                             // quad_perm 2 3 0 1
+    v += dpp<0x141>(v);                                            // row_half_mirror
+    if constexpr (LE >= 16) v += dpp<0x140>(v);                    // row_mirror
+    if constexpr (LE >= 32) {
+        const unsigned u = __builtin_bit_cast(unsigned, v);
+        const auto r = __builtin_amdgcn_permlane16_swap(u, u, false, false);
+        v = __builtin_bit_cast(float, (unsigned)r[0]) + __builtin_bit_cast(float, (unsigned)r[1]);
+    }
+    if constexpr (LE >= 64) {
+        const unsigned u = __builtin_bit_cast(unsigned, v);
+        const auto r = __builtin_amdgcn_permlane32_swap(u, u, false, false);
+        v = __builtin_bit_cast(float, (unsigned)r[0]) + __builtin_bit_cast(float, (unsigned)r[1]);
+    }
+    return v;
+}
+
 template <class T, int R, int LE>
 __global__ __launch_bounds__(256) void attn_rows_kernel(krk_attention_args a, int blocks_h, int splits, int span) {
     constexpr int V = VecOf<T>::V, KPW = 64 / LE, UK = 4;
@@ -41,48 +63,95 @@ __global__ __launch_bounds__(256) void attn_rows_kernel(krk_attention_args a, in
     const T* kp = (const T*)a.k + n * a.k_n + hk * a.k_h + e0;
     const T* vp = (const T*)a.v + n * a.v_n + hk * a.v_h + e0;
     const int j0 = blockIdx.y * span, j1 = min(j0 + span, row.limit);
-    for (int jb = j0 + wave * KPW * UK; jb < j1; jb += 4 * KPW * UK) {
-        bool in[UK];
-        float kv[UK][V], vv[UK][V], s[UK][R];
+    typedef T Tv __attribute__((ext_vector_type(V)));
+    Tv kr[UK], vr[UK];
+    unsigned in = 0;                                               // which of the keys in flight are seen, a bit each
+    auto fetch = [&](int jb) {                                     // nothing is loaded for a key that is not seen, whatever stands there
+        in = 0;
 #pragma unroll
         for (int u = 0; u < UK; ++u) {
             const int j = jb + u * KPW + grp;
-            in[u] = j < j1 && (!docs || docs[j] == doc);
-            load_vec<T, V>(kp + (long)(in[u] ? j : 0) * a.k_t, in[u] ? nv : 0, kv[u]);
-            load_vec<T, V>(vp + (long)(in[u] ? j : 0) * a.v_t, in[u] ? nv : 0, vv[u]);
+            const bool see = j < j1 && (!docs || docs[j] == doc);
+            kr[u] = vr[u] = (Tv)(T)0.f;
+            if (!see) continue;
+            in |= 1u << u;
+            if (nv >= V) {
+                __builtin_memcpy(&kr[u], kp + (long)j * a.k_t, sizeof(Tv));
+                __builtin_memcpy(&vr[u], vp + (long)j * a.v_t, sizeof(Tv));
+            } else {
+#pragma unroll
+                for (int v = 0; v < V; ++v)
+                    if (v < nv) kr[u][v] = kp[(long)j * a.k_t + v], vr[u][v] = vp[(long)j * a.v_t + v];
+            }
         }
+    };
+    constexpr int STEP = 4 * KPW * UK;
+    int jb = j0 + wave * KPW * UK;
+    if (jb < j1) fetch(jb);
+    for (; jb < j1; jb += STEP) {
+        Tv kc[UK], vc[UK];
+        const unsigned now = in;
+#pragma unroll
+        for (int u = 0; u < UK; ++u) kc[u] = kr[u], vc[u] = vr[u];
+        if (jb + STEP < j1) fetch(jb + STEP);                      // the next keys are in flight while these are used
+        float s[UK][R];
 #pragma unroll
         for (int u = 0; u < UK; ++u)
 #pragma unroll
             for (int r = 0; r < R; ++r) {
                 float d = 0.f;
 #pragma unroll
-                for (int v = 0; v < V; ++v) d = __builtin_fmaf(q[r][v], kv[u][v], d);
+                for (int v = 0; v < V; ++v) d = __builtin_fmaf(q[r][v], to_f<T>(kc[u][v]), d);
+                s[u][r] = group_sum<LE>(d);
+            }
+        if (a.cap > 0.f)
 #pragma unroll
-                for (int x = 1; x < LE; x <<= 1) d += __shfl_xor(d, x);
-                if (a.cap > 0.f) d = seq_cap<T>(d, a.cap, rcap) * LOG2E;
-                if (a.slopes) d = __builtin_fmaf(-slope[r], fabsf((float)(row.p - (jb + u * KPW + grp))), d);
-                s[u][r] = in[u] ? d : -INFINITY;
+            for (int u = 0; u < UK; ++u)
+#pragma unroll
+                for (int r = 0; r < R; ++r) s[u][r] = seq_cap<T>(s[u][r], a.cap, rcap) * LOG2E;
+        if (a.slopes)
+#pragma unroll
+            for (int u = 0; u < UK; ++u)
+#pragma unroll
+                for (int r = 0; r < R; ++r) s[u][r] = __builtin_fmaf(-slope[r], fabsf((float)(row.p - (jb + u * KPW + grp))), s[u][r]);
+        float top[R];
+        bool move = false;
+#pragma unroll
+        for (int r = 0; r < R; ++r) {
+            top[r] = -INFINITY;
+#pragma unroll
+            for (int u = 0; u < UK; ++u) {
+                s[u][r] = (now >> u) & 1u ? s[u][r] : -INFINITY;
+                top[r] = fmaxf(top[r], s[u][r]);
+            }
+            move = move || top[r] > m[r] + 8.f;
+        }
+        if (__ballot(move))                                        // as in the tile kernel: the reference point moves when a score passes it by 2^8
+#pragma unroll
+            for (int r = 0; r < R; ++r) {
+                const float nm = fmaxf(m[r], top[r]), f = __builtin_amdgcn_exp2f(m[r] - (nm == -INFINITY ? 0.f : nm));
+                m[r] = nm;
+                l[r] *= f;
+#pragma unroll
+                for (int v = 0; v < V; ++v) o[r][v] *= f;
             }
 #pragma unroll
         for (int r = 0; r < R; ++r) {
-            float top = m[r];
-#pragma unroll
-            for (int u = 0; u < UK; ++u) top = fmaxf(top, s[u][r]);
-            const float ref = top == -INFINITY ? 0.f : top;
-            const float f = __builtin_amdgcn_exp2f(m[r] - ref);
-            m[r] = top;
-            l[r] *= f;
-#pragma unroll
-            for (int v = 0; v < V; ++v) o[r][v] *= f;
+            const float ref = m[r] == -INFINITY ? 0.f : m[r];
 #pragma unroll
             for (int u = 0; u < UK; ++u) {
-                const float p = __builtin_amdgcn_exp2f(s[u][r] - ref);
-                l[r] += p;
-#pragma unroll
-                for (int v = 0; v < V; ++v) o[r][v] = __builtin_fmaf(p, vv[u][v], o[r][v]);
+                s[u][r] = __builtin_amdgcn_exp2f(s[u][r] - ref);
+                l[r] += s[u][r];
             }
         }
+#pragma unroll
+        for (int u = 0; u < UK; ++u)
+#pragma unroll
+            for (int v = 0; v < V; ++v) {
+                const float x = to_f<T>(vc[u][v]);
+#pragma unroll
+                for (int r = 0; r < R; ++r) o[r][v] = __builtin_fmaf(s[u][r], x, o[r][v]);
+            }
     }
     // join the groups of a wave, then the four waves
     __shared__ float wm[4][R], wl[4][R], wo[4][R][LE * V];
@@ -132,24 +201,38 @@ __global__ __launch_bounds__(256) void attn_rows_kernel(krk_attention_args a, in
     }
 }
 
-// joins the splits of one row: a wave per row, lanes along E
+constexpr int MAX_SPLITS = 64;
+
+// joins the splits of one row: a wave per row, lanes along the splits for their weights, along E for the sums
 template <class T>
 __global__ __launch_bounds__(256) void attn_join_kernel(krk_attention_args a, int splits, long rows) {
     const long row = (long)blockIdx.x * 4 + (threadIdx.x >> 6);
     if (row >= rows) return;
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+    __shared__ float weight[4][MAX_SPLITS];
     const float* ws = (const float*)a.workspace;
-    const float* ml = ws + rows * splits * a.E + row * splits * 2;
+    const float2* ml = (const float2*)(ws + rows * splits * a.E) + row * splits;
     float top = -INFINITY, sum = 0.f;
-    for (int x = 0; x < splits; ++x) top = fmaxf(top, ml[2 * x]);
+    for (int x = lane; x < splits; x += 64) top = fmaxf(top, ml[x].x);
+#pragma unroll
+    for (int x = 1; x < 64; x <<= 1) top = fmaxf(top, __shfl_xor(top, x));
     const float ref = top == -INFINITY ? 0.f : top;
-    for (int x = 0; x < splits; ++x) sum = __builtin_fmaf(ml[2 * x + 1], __builtin_amdgcn_exp2f(ml[2 * x] - ref), sum);
+    for (int x = lane; x < splits; x += 64) {
+        const float w = __builtin_amdgcn_exp2f(ml[x].x - ref);
+        weight[wave][x] = w;
+        sum = __builtin_fmaf(ml[x].y, w, sum);
+    }
+#pragma unroll
+    for (int x = 1; x < 64; x <<= 1) sum += __shfl_xor(sum, x);
+    __builtin_amdgcn_wave_barrier();                               // a wave reads what it wrote itself
     const int h = row % a.H;
     const long it = row / a.H;
     const int i = it % a.Tq;
     const long n = it / a.Tq;
-    for (int e = threadIdx.x & 63; e < a.E; e += 64) {
+    for (int e = lane; e < a.E; e += 64) {
         float t = 0.f;
-        for (int x = 0; x < splits; ++x) t = __builtin_fmaf(ws[(row * splits + x) * a.E + e], __builtin_amdgcn_exp2f(ml[2 * x] - ref), t);
+#pragma unroll 8
+        for (int x = 0; x < splits; ++x) t = __builtin_fmaf(ws[(row * splits + x) * a.E + e], weight[wave][x], t);
         ((T*)a.out)[n * a.o_n + i * a.o_t + h * a.o_h + e] = from_f<T>(sum == 0.f ? 0.f : t / sum);
     }
 }
@@ -159,13 +242,13 @@ int row_block(const krk_attention_args& a) {
     return rep >= 8 ? 8 : rep >= 4 ? 4 : rep >= 2 ? 2 : 1;
 }
 
-// workgroups along the key axis: enough for four per CU where there are few rows, 256 keys at least for each
+// workgroups along the key axis: enough for eight per CU where there are few rows, 256 keys at least for each
 int split_count(const krk_attention_args& a) {
     const int rep = a.H / a.Hk, R = row_block(a);
     const long items = (long)a.N * a.Tq * a.Hk * ((rep + R - 1) / R);
     if (items <= 0 || a.Tk <= 0) return 1;
-    long want = (1024 + items - 1) / items, most = (a.Tk + 255) / 256;
-    return (int)max(1L, min(min(want, most), 1024L));
+    long want = (2048 + items - 1) / items, most = (a.Tk + 255) / 256;
+    return (int)max(1L, min(min(want, most), (long)MAX_SPLITS));
 }
 
 template <class T, int R, int LE>
