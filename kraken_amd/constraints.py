@@ -11,7 +11,7 @@ import numpy as np
 import torch
 
 from . import _lib
-from .sequence import _TYPES, _call, _first, _lengths, _like, _ptr
+from .sequence import _TYPES, _call, _first, _lengths, _like, _own_memory, _ptr
 
 __all__ = ['constrain_logits', 'label_mask']
 
@@ -98,14 +98,13 @@ def constrain_logits(logits: torch.Tensor, *, mask: Optional[torch.Tensor] = Non
     elif history_lens is not None:
         raise ValueError('history_lens without history')
     if out is None:
-        y = torch.empty(x.shape, dtype=x.dtype, device=x.device)
+        y = x.new_empty(x.shape)
         result = y.squeeze(1) if step else y
     else:
         if _like(out, 'out', shape, x) is not out:
             raise ValueError('out is written in place: its classes have to be adjacent')
         result, y = out, out.unsqueeze(1) if step else out
         same = y.data_ptr() == x.data_ptr() and all(i == j or s == 1 for i, j, s in zip(y.stride(), x.stride(), x.shape))
-        from .sequence import _own_memory
         _own_memory(y, 'out', (None if same else x, mask, bias, history, lens, rep[0], pres[0], freq[0]))
     if n == 0 or t == 0 or c == 0:
         return result

@@ -33,8 +33,8 @@ template <int LE> __device__ __forceinline__ float group_sum(float v) {
 }
 
 template <class T, int R, int LE>
-__global__ __launch_bounds__(256) void attn_rows_kernel(krk_attention_args a, int blocks_h, int splits, int span) {
-    constexpr int V = VecOf<T>::V, KPW = 64 / LE, UK = 4;
+__global__ __launch_bounds__(256, R == 8 ? 2 : sizeof(T) == 2 ? 3 : 1) void attn_rows_kernel(krk_attention_args a, int blocks_h, int splits, int span) {
+    constexpr int V = VecOf<T>::V, KPW = 64 / LE, UK = R == 8 ? 2 : 4;
     const int rep = a.H / a.Hk;
     long item = blockIdx.x;
     const int rb = item % blocks_h; item /= blocks_h;

@@ -2648,6 +2648,12 @@ int krk_upsample_sigmoid(const float* x_dev, int C, int h, int w, int H, int W, 
 }
 
 // ---- operators on sequence rows (conv_seq.hip, scan_seq.hip, attn_seq.hip, constrain.hip)
+// whether there is a device at all: asked once, these calls are short
+static bool seq_device() {
+    static const bool there = krk_device_count() > 0;
+    return there;
+}
+
 static bool seq_type(int t) { return t == KRK_TYPE_F32 || t == KRK_TYPE_BF16 || t == KRK_TYPE_F16; }
 
 // the common end of an operator: its launcher's answer as an error code
@@ -2662,7 +2668,7 @@ int krk_causal_conv(const krk_conv_args* a, void* stream) {
         return fail(KRK_E_INVALID, "krk_causal_conv: bad argument");
     if (a->K < 1 || a->K > 8) return fail(KRK_E_UNSUPPORTED, "krk_causal_conv: kernels of 1 to 8 steps");
     if (a->state_out && a->state_out == a->state && a->T != 1) return fail(KRK_E_INVALID, "krk_causal_conv: in place for one step only");
-    if (krk_device_count() <= 0) return fail(KRK_E_HIP, "krk_causal_conv: no HIP device");
+    if (!seq_device()) return fail(KRK_E_HIP, "krk_causal_conv: no HIP device");
     if (a->N == 0 || (a->T == 0 && !a->state_out)) return KRK_OK;
     return seq_done("krk_causal_conv", krk_launch_causal_conv(*a, (hipStream_t)stream));
 }
@@ -2683,7 +2689,7 @@ long krk_selective_scan_workspace(const krk_scan_args* a) {
 
 int krk_selective_scan(const krk_scan_args* a, void* stream) {
     if (int rc = scan_args_ok(a)) return rc;
-    if (krk_device_count() <= 0) return fail(KRK_E_HIP, "krk_selective_scan: no HIP device");
+    if (!seq_device()) return fail(KRK_E_HIP, "krk_selective_scan: no HIP device");
     if (a->N == 0 || (a->T == 0 && !a->state_out)) return KRK_OK;
     const long need = krk_scan_workspace(*a);
     if (need > 0 && (!a->workspace || a->workspace_bytes < need)) return fail(KRK_E_INVALID, "krk_selective_scan: workspace too small");
@@ -2707,7 +2713,7 @@ long krk_attention_workspace(const krk_attention_args* a) {
 
 int krk_attention(const krk_attention_args* a, void* stream) {
     if (int rc = attention_args_ok(a)) return rc;
-    if (krk_device_count() <= 0) return fail(KRK_E_HIP, "krk_attention: no HIP device");
+    if (!seq_device()) return fail(KRK_E_HIP, "krk_attention: no HIP device");
     if (a->N == 0 || a->Tq == 0) return KRK_OK;
     const long need = krk_attn_workspace(*a);
     if (need > 0 && (!a->workspace || a->workspace_bytes < need)) return fail(KRK_E_INVALID, "krk_attention: workspace too small");
@@ -2717,7 +2723,7 @@ int krk_attention(const krk_attention_args* a, void* stream) {
 int krk_constrain_logits(const krk_constrain_args* a, void* stream) {
     if (!a || !a->logits || !a->out || a->N < 0 || a->T < 0 || a->C <= 0 || a->L < 0 || !seq_type(a->type))
         return fail(KRK_E_INVALID, "krk_constrain_logits: bad argument");
-    if (krk_device_count() <= 0) return fail(KRK_E_HIP, "krk_constrain_logits: no HIP device");
+    if (!seq_device()) return fail(KRK_E_HIP, "krk_constrain_logits: no HIP device");
     if (a->N == 0 || a->T == 0) return KRK_OK;
     return seq_done("krk_constrain_logits", krk_launch_constrain(*a, (hipStream_t)stream));
 }

@@ -43,10 +43,14 @@ def _first(x, name, dim):
 
 def _like(t, name, shape, first, dtype=None, inner=1):
     """A tensor that goes with `first`: shape, type (first's unless given), device; its last `inner` axes adjacent (else a copy)."""
+    if dtype is None:
+        dtype = first.dtype
+    if isinstance(t, torch.Tensor) and t.shape == shape and t.dtype is dtype and t.device == first.device and not t.requires_grad and t.is_contiguous():
+        return t                                    # what a step of a stream passes, in one condition: it is called for every label
     if not isinstance(t, torch.Tensor) or t.shape != shape:
         raise ValueError(f'{name} has to be a tensor of shape {tuple(shape)}, got {tuple(t.shape) if isinstance(t, torch.Tensor) else type(t)}')
-    if t.dtype != (dtype or first.dtype):
-        raise ValueError(f'{name} has to be {dtype or first.dtype}, not {t.dtype}')
+    if t.dtype != dtype:
+        raise ValueError(f'{name} has to be {dtype}, not {t.dtype}')
     if t.device != first.device:
         raise ValueError(f'{name} is on {t.device}, the call on {first.device}')
     if t.requires_grad and torch.is_grad_enabled():
@@ -81,12 +85,13 @@ def _lengths(lens, name, n, top, dev):
 
 def _own_memory(t, name, others):
     """A tensor that a call updates in place: no element twice, and nothing shared with the inputs."""
-    spans = sorted((st, sz) for st, sz in zip(t.stride(), t.shape) if sz > 1)
-    end = 1
-    for st, sz in spans:
-        if st < end:
-            raise ValueError(f'{name} overlaps itself: it is updated in place')
-        end += (sz - 1) * st
+    end = t.numel()
+    if not t.is_contiguous():
+        end = 1
+        for st, sz in sorted((st, sz) for st, sz in zip(t.stride(), t.shape) if sz > 1):
+            if st < end:
+                raise ValueError(f'{name} overlaps itself: it is updated in place')
+            end += (sz - 1) * st
     lo = t.data_ptr()
     hi = lo + end * t.element_size()
     for o in others:
@@ -98,13 +103,21 @@ def _ptr(t):
     return None if t is None else t.data_ptr()
 
 
+def _current_stream(dev):
+    return torch.cuda.current_stream(dev).cuda_stream
+
+
+# the handle alone, without an object around it: a third of what a step costs the host otherwise
+_raw_stream = getattr(torch._C, '_cuda_getCurrentRawStream', None)
+
+
 def _call(fn, args, dev):
     """The entry point on the device's current stream; a device that is not the current one is made it for the launch."""
     if dev.index == torch.cuda.current_device():
-        rc = fn(C.byref(args), torch.cuda.current_stream(dev).cuda_stream)
+        rc = fn(C.byref(args), _raw_stream(dev.index) if _raw_stream else _current_stream(dev))
     else:
         with torch.cuda.device(dev):
-            rc = fn(C.byref(args), torch.cuda.current_stream(dev).cuda_stream)
+            rc = fn(C.byref(args), _current_stream(dev))
     if rc:
         _lib.check(rc)
 
@@ -143,8 +156,8 @@ def causal_conv(x: torch.Tensor, weight: torch.Tensor, bias: Optional[torch.Tens
     lens = _lengths(seq_lens, 'seq_lens', n, t, x.device)
     if state is not None:
         state = _like(state, 'state', (n, k - 1, d), x)
-    y = torch.empty((n, t, d), dtype=x.dtype, device=x.device)
-    out = torch.empty((n, k - 1, d), dtype=x.dtype, device=x.device)
+    y = x.new_empty((n, t, d))
+    out = x.new_empty((n, k - 1, d))
     if n == 0 or d == 0 or t == 0:
         return y, out.zero_() if state is None else out.copy_(state)
     has = k > 1
@@ -167,7 +180,7 @@ def causal_conv_step(x: torch.Tensor, weight: torch.Tensor, bias: Optional[torch
     silu = _silu(activation)
     if _like(state, 'state', (n, k - 1, d), x) is not state:
         raise ValueError('state is updated in place: its channels have to be adjacent')
-    y = torch.empty((n, d), dtype=x.dtype, device=x.device)
+    y = x.new_empty((n, d))
     if n == 0 or d == 0:
         return y
     at = None
@@ -220,7 +233,7 @@ def selective_scan(x: torch.Tensor, dt: torch.Tensor, A: torch.Tensor, B: torch.
     lens = _lengths(seq_lens, 'seq_lens', n, t, x.device)
     if state is not None:
         state = _like(state, 'state', (n, d, s), x, torch.float32, 2)
-    y = torch.empty((n, t, d), dtype=x.dtype, device=x.device)
+    y = x.new_empty((n, t, d))
     out = torch.empty((n, d, s), dtype=torch.float32, device=x.device)
     if n == 0 or d == 0 or t == 0:
         return y, out.zero_() if state is None else out.copy_(state)
@@ -247,7 +260,7 @@ def selective_scan_step(x: torch.Tensor, dt: torch.Tensor, A: torch.Tensor, B: t
     dt, A, B, C, D, z, dt_bias, s, g = _scan_args(x, dt, A, B, C, D, z, dt_bias)
     if _like(state, 'state', (n, d, s), x, torch.float32, 2) is not state:
         raise ValueError('state is updated in place: the states of a line have to be adjacent')
-    y = torch.empty((n, d), dtype=x.dtype, device=x.device)
+    y = x.new_empty((n, d))
     if n == 0 or d == 0:
         return y
     _own_memory(state, 'state', (x, dt, A, B, C, D, z, dt_bias))
@@ -318,7 +331,7 @@ def attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, seq_lens: Lens 
     if slopes is not None:
         slopes = _like(slopes, 'slopes', (h,), q, torch.float32)
     cap, scale = _finite(cap, 'cap', 0), e ** -0.5 if scale is None else _finite(scale, 'scale', -math.inf)
-    out = torch.empty((n, tq, h, e), dtype=q.dtype, device=dev)
+    out = q.new_empty((n, tq, h, e))
     if n == 0 or tq == 0:
         return out
     if tk == 0:
