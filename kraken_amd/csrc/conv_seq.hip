@@ -14,6 +14,7 @@ constexpr int U = 4;          // steps whose loads are in flight together
 template <class T, int K>
 __global__ __launch_bounds__(256) void conv_seq_kernel(krk_conv_args a, int groups, int runs, int steps) {
     constexpr int V = VecOf<T>::V, W = K - 1;
+    typedef T Raw __attribute__((ext_vector_type(V)));
     const int id = blockIdx.x * 256 + threadIdx.x;
     const int run = id / groups, d0 = (id - run * groups) * V;
     if (run >= runs) return;
@@ -39,7 +40,17 @@ __global__ __launch_bounds__(256) void conv_seq_kernel(krk_conv_args a, int grou
 #pragma unroll
                 for (int j = 0; j < V; ++j) v[j] = 0.f;
         };
-        const int i0 = run * steps, i1 = min(i0 + steps, a.T);
+        const int i0 = run * steps, i1 = min(i0 + steps, a.T), end = min(i1, len);
+        Raw next[U];
+        // the next U steps, behind the end the last one again: loads without a condition, in flight while the steps before them are computed
+        auto fetch = [&](int i) {
+#pragma unroll
+            for (int u = 0; u < U; ++u) {
+                const int k = min(i + u, end - 1);
+                next[u] = load_raw<T, V>(x + (long)(a.reverse ? len - 1 - k : k) * a.x_t, nv);
+            }
+        };
+        if (i0 < end) fetch(i0);
         float win[W + U][V];
 #pragma unroll
         for (int k = 0; k < W; ++k)
@@ -51,14 +62,14 @@ __global__ __launch_bounds__(256) void conv_seq_kernel(krk_conv_args a, int grou
 #pragma unroll
             for (int k = 0; k < W; ++k) store_vec<T, V>((T*)a.state_out + n * a.out_n + k * a.out_k + d0, nv, last[k]);
         }
-        int i = i0;
-        for (; i < min(i1, len); i += U) {
+        for (int i = i0; i < end; i += U) {
 #pragma unroll
             for (int u = 0; u < U; ++u)
-                if (i + u < min(i1, len)) input(i + u, win[W + u]);
+#pragma unroll
+                for (int j = 0; j < V; ++j) win[W + u][j] = to_f<T>(next[u][j]);
+            if (i + U < end) fetch(i + U);
 #pragma unroll
             for (int u = 0; u < U; ++u) {
-                if (i + u >= min(i1, len)) break;
                 float p[V];
 #pragma unroll
                 for (int j = 0; j < V; ++j) {
@@ -67,7 +78,7 @@ __global__ __launch_bounds__(256) void conv_seq_kernel(krk_conv_args a, int grou
                     for (int k = 0; k < K; ++k) s = __builtin_fmaf(w[k][j], win[u + k][j], s);
                     p[j] = a.silu ? seq_silu(s) : s;
                 }
-                store_vec<T, V>(y + (long)(a.reverse ? len - 1 - (i + u) : i + u) * a.y_t, nv, p);
+                if (i + u < end) store_vec<T, V>(y + (long)(a.reverse ? len - 1 - (i + u) : i + u) * a.y_t, nv, p);
             }
 #pragma unroll
             for (int k = 0; k < W; ++k)

@@ -26,6 +26,17 @@ template <class T, int V> __device__ __forceinline__ void load_vec(const T* p, i
         for (int i = 0; i < V; ++i) v[i] = i < nv ? to_f<T>(p[i]) : 0.f;
     }
 }
+// the same without the conversion, for loads that are to stay in flight
+template <class T, int V> __device__ __forceinline__ auto load_raw(const T* p, int nv) {
+    typedef T Tv __attribute__((ext_vector_type(V)));
+    Tv t = (Tv)(T)0.f;
+    if (nv >= V) __builtin_memcpy(&t, p, sizeof(T) * V);
+    else
+#pragma unroll
+        for (int i = 0; i < V; ++i)
+            if (i < nv) t[i] = p[i];
+    return t;
+}
 template <class T, int V> __device__ __forceinline__ void store_vec(T* p, int nv, const float (&v)[V]) {
     typedef T Tv __attribute__((ext_vector_type(V)));
     if (nv >= V) {
