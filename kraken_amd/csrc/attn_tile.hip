@@ -23,22 +23,21 @@ __device__ __forceinline__ f32x16 mfma16(f16_t, const s16x8& a, const s16x8& b, 
 }
 __device__ __forceinline__ f32x16 mfma16(float, const s16x8&, const s16x8&, const f32x16& c) { return c; }
 
-// The 16 bytes of a head from channel e on, zeros behind its end (E channels, 16 bytes at least).  The last, partial one is loaded so that it ENDS
-// there: one load without a condition whatever E is, and none past the row; place_chunk moves it into place, apart from the load, so that
-// nothing waits for the load before it has to.
-typedef unsigned long long u64x2 __attribute__((ext_vector_type(2)));
+// A head is read in chunks of 16 bytes; where its E channels are no whole number of them, the last chunk is loaded so that it ENDS there: one load
+// without a condition whatever E is, and none past the row.  Its first channels are in the chunk before as well: keys and values are kept so,
+// the query has zeros in their place, and the result of such a channel is stored once.  Chunks behind the last repeat it, the query zero.
 template <class T> __device__ __forceinline__ u32x4 load_chunk(const T* row, int e, int E) {
     u32x4 r;
     __builtin_memcpy(&r, row + min(e, E - VecOf<T>::V), 16);
     return r;
 }
-template <class T> __device__ __forceinline__ u32x4 place_chunk(u32x4 r, int e, int E) {
-    const int sh = max(0, (e + VecOf<T>::V - E) * (int)sizeof(T) * 8);
-    u64x2 w = __builtin_bit_cast(u64x2, r);
-    w[0] = sh >= 64 ? w[1] >> (sh & 63) : sh ? w[0] >> sh | w[1] << (64 - sh) : w[0];
-    w[1] = sh >= 64 ? 0 : w[1] >> sh;
-    if (sh >= 128) w[0] = 0;
-    return __builtin_bit_cast(u32x4, w);
+// the query's chunk at e: without the channels that the chunk before has, and nothing behind the end
+template <class T> __device__ __forceinline__ u32x4 query_chunk(u32x4 r, int e, int E) {
+    typedef T Tv __attribute__((ext_vector_type(VecOf<T>::V)));
+    Tv v = __builtin_bit_cast(Tv, r);
+#pragma unroll
+    for (int i = 0; i < VecOf<T>::V; ++i) v[i] = i >= e - (E - VecOf<T>::V) && e < E ? v[i] : (T)0.f;
+    return __builtin_bit_cast(u32x4, v);
 }
 
 // the lane 32 away: a query's keys lie in two lanes
@@ -96,6 +95,15 @@ __global__ __launch_bounds__(256) void attn_ranges_kernel(krk_attention_args a, 
 #pragma unroll
     for (int x = 1; x < 64; x <<= 1) lo = min(lo, __shfl_xor(lo, x)), hi = max(hi, __shfl_xor(hi, x));
     if (lane == 0) out[id] = make_int2(lo, hi);
+}
+
+// four channels at p, the first `from` of which are stored already
+template <class T> __device__ __forceinline__ void put_four(T* p, int from, const float (&v)[4]) {
+    if (from == 0) store_vec<T, 4>(p, 4, v);
+    else
+#pragma unroll
+        for (int i = 1; i < 4; ++i)
+            if (i >= from) p[i] = from_f<T>(v[i]);
 }
 
 // a statement for every score of a lane: s[x][i]
@@ -164,23 +172,12 @@ __global__ __launch_bounds__(NW * 64, EP * sizeof(T) > 256 ? 1 : 2) void attn_ti
     const float c = (a.scale != 0.f ? fabsf(a.scale) : 1.f) * LOG2E;
     s16x8 q16[F32 ? 1 : EP / 16];
     f32x4 q32[F32 ? EP / 8 : 1];
+    constexpr int NQ = F32 ? EP / 8 : EP / 16, STEP = F32 ? 8 : 16;
+    u32x4 raw[NQ];
     {
         const T* qp = (const T*)a.q + n * a.q_n + (long)min(qi, a.Tq - 1) * a.q_t + h * a.q_h;
-        constexpr int NQ = F32 ? EP / 8 : EP / 16, STEP = F32 ? 8 : 16;
-        u32x4 raw[NQ];
 #pragma unroll
         for (int x = 0; x < NQ; ++x) raw[x] = load_chunk<T>(qp, STEP * x + STEP / 2 * half, a.E);
-#pragma unroll
-        for (int x = 0; x < NQ; ++x) {
-            if (a.E != EP) raw[x] = place_chunk<T>(raw[x], STEP * x + STEP / 2 * half, a.E);
-            if constexpr (F32) q32[x] = __builtin_bit_cast(f32x4, raw[x]) * sign;
-            else {
-                q16[x] = __builtin_bit_cast(s16x8, raw[x]);
-                if (a.scale <= 0.f)
-#pragma unroll
-                    for (int i = 0; i < 8; ++i) q16[x][i] = __builtin_bit_cast(short, from_f<T>(to_f(__builtin_bit_cast(T, q16[x][i])) * sign));
-            }
-        }
     }
     const float slope = a.slopes ? a.slopes[h] * LOG2E : 0.f;
     const float rcap = a.cap > 0.f ? 1.f / a.cap : 0.f;
@@ -238,13 +235,6 @@ __global__ __launch_bounds__(NW * 64, EP * sizeof(T) > 256 ? 1 : 2) void attn_ti
     auto search = [&](int t) { return docs || (t + 1) * BK > bmin; };
     auto put = [&](int t, int buf, int turn) {
         unsigned high = 0;
-        if (a.E != EP)
-#pragma unroll
-            for (int x = 0; x < CPT; ++x) {
-                const int e = (threadIdx.x + x * NT) % CPR * CV;
-                kr[x] = place_chunk<T>(kr[x], e, a.E);
-                vr[x] = place_chunk<T>(vr[x], e, a.E);
-            }
 #pragma unroll
         for (int x = 0; x < CPT; ++x)
 #pragma unroll
@@ -278,10 +268,19 @@ __global__ __launch_bounds__(NW * 64, EP * sizeof(T) > 256 ? 1 : 2) void attn_ti
     __syncthreads();
     int tile = next(), turn = 0;
     bool was = false;
-    if (tile >= 0) {
-        fetch(tile);
-        put(tile, 0, 0);
+    if (tile >= 0) fetch(tile);
+#pragma unroll
+    for (int x = 0; x < NQ; ++x) {
+        if (a.E != EP) raw[x] = query_chunk<T>(raw[x], STEP * x + STEP / 2 * half, a.E);
+        if constexpr (F32) q32[x] = __builtin_bit_cast(f32x4, raw[x]) * sign;
+        else {
+            q16[x] = __builtin_bit_cast(s16x8, raw[x]);
+            if (a.scale <= 0.f)
+#pragma unroll
+                for (int i = 0; i < 8; ++i) q16[x][i] = __builtin_bit_cast(short, from_f<T>(to_f(__builtin_bit_cast(T, q16[x][i])) * sign));
+        }
     }
+    if (tile >= 0) put(tile, 0, 0);
     __builtin_amdgcn_s_waitcnt(0x0f70);                                   // vmcnt(0): nothing of the prologue is waited for behind the loop's own loads
     __syncthreads();
     while (tile >= 0) {
@@ -430,32 +429,37 @@ __global__ __launch_bounds__(NW * 64, EP * sizeof(T) > 256 ? 1 : 2) void attn_ti
 
     l = other_half_sum(l);
     if (qi >= a.Tq) return;
-    if (splits == 1) {
-        const float r = lim > 0 && l != 0.f ? 1.f / l : 0.f;
+    // four neighbouring rows of O^T at a time: their channel, and how many of them the chunk before has stored
+    auto each_four = [&](auto store) {
 #pragma unroll
         for (int eb = 0; eb < EB; ++eb)
 #pragma unroll
             for (int g = 0; g < 4; ++g) {
-                const int e = eb * 32 + 8 * g + 4 * half;
+                const int e = eb * 32 + 8 * g + 4 * half, chunk = e / CV * CV;        // O^T's rows lie as the chunks of V do
+                if (chunk >= a.E) continue;
+                const int shift = max(0, chunk - (a.E - CV)), from = min(4, max(0, shift - (e - chunk)));
                 float v[4];
 #pragma unroll
-                for (int i = 0; i < 4; ++i) v[i] = lim > 0 && l != 0.f ? o[eb][4 * g + i] * r : 0.f;
-                store_vec<T, 4>(out + (long)qi * a.o_t + e, a.E - e, v);
+                for (int i = 0; i < 4; ++i) v[i] = o[eb][4 * g + i];
+                store(e - shift, from, v);
             }
+    };
+    if (splits == 1) {
+        const float r = lim > 0 && l != 0.f ? 1.f / l : 0.f;
+        each_four([&](int e, int from, float (&v)[4]) {
+#pragma unroll
+            for (int i = 0; i < 4; ++i) v[i] = lim > 0 && l != 0.f ? v[i] * r : 0.f;
+            put_four<T>(out + (long)qi * a.o_t + e, from, v);
+        });
     } else {
         float* ws = (float*)((char*)a.workspace);
         const long rows = (long)a.N * a.Tq * a.H, at = (((long)n * a.Tq + qi) * a.H + h) * splits + split;
         const bool any = lim > 0;
+        each_four([&](int e, int from, float (&v)[4]) {
 #pragma unroll
-        for (int eb = 0; eb < EB; ++eb)
-#pragma unroll
-            for (int g = 0; g < 4; ++g) {
-                const int e = eb * 32 + 8 * g + 4 * half;
-                float v[4];
-#pragma unroll
-                for (int i = 0; i < 4; ++i) v[i] = any ? o[eb][4 * g + i] : 0.f;
-                store_vec<float, 4>(ws + at * a.E + e, a.E - e, v);
-            }
+            for (int i = 0; i < 4; ++i) v[i] = any ? v[i] : 0.f;
+            put_four<float>(ws + at * a.E + e, from, v);
+        });
         if (half == 0) {
             ws[rows * splits * a.E + at * 2] = any ? m : -INFINITY;
             ws[rows * splits * a.E + at * 2 + 1] = any ? l : 0.f;
