@@ -277,7 +277,10 @@ __global__ __launch_bounds__(NW * 64, EP * sizeof(T) > 256 ? 1 : 2) void attn_ti
             q16[x] = __builtin_bit_cast(s16x8, raw[x]);
             if (a.scale <= 0.f)
 #pragma unroll
-                for (int i = 0; i < 8; ++i) q16[x][i] = __builtin_bit_cast(short, from_f<T>(to_f(__builtin_bit_cast(T, q16[x][i])) * sign));
+                for (int i = 0; i < 8; ++i) {
+                    const short one = q16[x][i];                          // a copy: a bit cast of a vector's element reads its first one
+                    q16[x][i] = __builtin_bit_cast(short, from_f<T>(to_f(__builtin_bit_cast(T, one)) * sign));
+                }
         }
     }
     if (tile >= 0) put(tile, 0, 0);
@@ -472,6 +475,7 @@ int launch(const krk_attention_args& a, const AttnTiles& g, void* scratch, hipSt
     const int qblocks = (a.Tq + NW * 32 - 1) / (NW * 32), tiles = (a.Tk + g.keys - 1) / g.keys;
     const int2* ranges = nullptr;
     if (a.documents) {
+        if ((long)a.N * tiles > 0x7fffff00L) return -4;
         int2* r = (int2*)scratch;
         ranges = r;
         hipLaunchKernelGGL(attn_ranges_kernel, dim3((unsigned)(((long)a.N * tiles + 3) / 4)), dim3(256), 0, s, a, r, tiles, g.keys);

@@ -12,6 +12,7 @@
 #include <cstdio>
 #include <cstdlib>
 #include <cstring>
+#include <initializer_list>
 #include <map>
 #include <string>
 #include <memory>
@@ -2656,6 +2657,13 @@ static bool seq_device() {
 
 static bool seq_type(int t) { return t == KRK_TYPE_F32 || t == KRK_TYPE_BF16 || t == KRK_TYPE_F16; }
 
+// axes up to 2^30: the kernels count steps, channels and rows in int
+static bool seq_large(std::initializer_list<int> sizes) {
+    for (int n : sizes)
+        if (n > 1 << 30) return true;
+    return false;
+}
+
 // the common end of an operator: its launcher's answer as an error code
 static int seq_done(const char* who, int rc) {
     if (rc == -4) return fail(KRK_E_UNSUPPORTED, std::string(who) + ": more rows than one launch can address");
@@ -2667,6 +2675,7 @@ int krk_causal_conv(const krk_conv_args* a, void* stream) {
     if (!a || !a->x || !a->weight || !a->y || a->N < 0 || a->T < 0 || a->D <= 0 || !seq_type(a->type))
         return fail(KRK_E_INVALID, "krk_causal_conv: bad argument");
     if (a->K < 1 || a->K > 8) return fail(KRK_E_UNSUPPORTED, "krk_causal_conv: kernels of 1 to 8 steps");
+    if (seq_large({a->N, a->T, a->D})) return fail(KRK_E_UNSUPPORTED, "krk_causal_conv: axes up to 2^30");
     if (a->state_out && a->state_out == a->state && a->T != 1) return fail(KRK_E_INVALID, "krk_causal_conv: in place for one step only");
     if (!seq_device()) return fail(KRK_E_HIP, "krk_causal_conv: no HIP device");
     if (a->N == 0 || (a->T == 0 && !a->state_out)) return KRK_OK;
@@ -2677,6 +2686,7 @@ static int scan_args_ok(const krk_scan_args* a) {
     if (!a || !a->x || !a->dt || !a->A || !a->B || !a->C || !a->y || a->N < 0 || a->T < 0 || a->D <= 0 || !seq_type(a->type))
         return fail(KRK_E_INVALID, "krk_selective_scan: bad argument");
     if (a->S < 1 || a->S > 256) return fail(KRK_E_UNSUPPORTED, "krk_selective_scan: 1 to 256 states");
+    if (seq_large({a->N, a->T, a->D})) return fail(KRK_E_UNSUPPORTED, "krk_selective_scan: axes up to 2^30");
     if (a->G < 1 || a->D % a->G) return fail(KRK_E_INVALID, "krk_selective_scan: groups must divide the channels");
     if (a->state_out && a->state_out == a->state && a->T != 1) return fail(KRK_E_INVALID, "krk_selective_scan: in place for one step only");
     return KRK_OK;
@@ -2701,6 +2711,7 @@ static int attention_args_ok(const krk_attention_args* a) {
         return fail(KRK_E_INVALID, "krk_attention: bad argument");
     if (a->H % a->Hk) return fail(KRK_E_INVALID, "krk_attention: key heads must divide the query heads");
     if (a->E < 1 || a->E > 256) return fail(KRK_E_UNSUPPORTED, "krk_attention: heads of 1 to 256 channels");
+    if (seq_large({a->N, a->Tq, a->Tk, a->H})) return fail(KRK_E_UNSUPPORTED, "krk_attention: axes up to 2^30");
     if (a->documents && a->Tq != a->Tk) return fail(KRK_E_INVALID, "krk_attention: documents need as many queries as keys");
     if (!(a->cap >= 0.f)) return fail(KRK_E_INVALID, "krk_attention: cap must not be negative");
     return KRK_OK;
@@ -2723,6 +2734,7 @@ int krk_attention(const krk_attention_args* a, void* stream) {
 int krk_constrain_logits(const krk_constrain_args* a, void* stream) {
     if (!a || !a->logits || !a->out || a->N < 0 || a->T < 0 || a->C <= 0 || a->L < 0 || !seq_type(a->type))
         return fail(KRK_E_INVALID, "krk_constrain_logits: bad argument");
+    if (seq_large({a->N, a->T, a->C, a->L})) return fail(KRK_E_UNSUPPORTED, "krk_constrain_logits: axes up to 2^30");
     if (!seq_device()) return fail(KRK_E_HIP, "krk_constrain_logits: no HIP device");
     if (a->N == 0 || a->T == 0) return KRK_OK;
     return seq_done("krk_constrain_logits", krk_launch_constrain(*a, (hipStream_t)stream));

@@ -15,51 +15,54 @@ __global__ __launch_bounds__(256) void constrain_kernel(krk_constrain_args a, in
 #pragma clang fp contract(off)
     constexpr int V = VecOf<T>::V;
     __shared__ int count[CH];
-    const int n = blockIdx.z, c0 = blockIdx.x * CH, c1 = min(c0 + CH, a.C);
+    const int c0 = blockIdx.x * CH, c1 = min(c0 + CH, a.C);
     const bool hist = a.history != nullptr;
-    float rep = 1.f, pres = 0.f, freq = 0.f;
-    if (hist) {
-        rep = a.repetition ? a.repetition[n] : a.all_repetition;
-        pres = a.presence ? a.presence[n] : a.all_presence;
-        freq = a.frequency ? a.frequency[n] : a.all_frequency;
-        for (int i = threadIdx.x; i < c1 - c0; i += 256) count[i] = 0;
-        __syncthreads();
-        const int L = seq_len(a.hist_lens, n, a.L);
-        const I* h = (const I*)a.history + n * a.hist_n;
-        for (int i = threadIdx.x; i < L; i += 256) {
-            const I c = h[i];
-            if (c >= c0 && c < c1) atomicAdd(&count[(int)(c - c0)], 1);
-        }
-        __syncthreads();
-    }
-    const int tx = threadIdx.x & ((1 << tx_bits) - 1), ty = threadIdx.x >> tx_bits;
-    const int t1 = min((int)(blockIdx.y + 1) * rows, a.T);
-    for (int t = blockIdx.y * rows + ty; t < t1; t += 256 >> tx_bits) {
-        const T* in = (const T*)a.logits + n * a.l_n + t * a.l_t;
-        T* out = (T*)a.out + n * a.o_n + t * a.o_t;
-        const unsigned* mask = a.mask ? a.mask + n * a.mask_n + t * a.mask_t : nullptr;
-        for (int c = c0 + tx * V; c < c1; c += V << tx_bits) {
-            const int nv = min(V, c1 - c);
-            float v[V], b[V];
-            load_vec<T, V>(in + c, nv, v);
-            const unsigned bits = mask ? mask[c >> 5] >> (c & 31) : ~0u;
-            if (a.bias) load_vec<float, V>(a.bias + n * a.bias_n + c, nv, b);
-#pragma unroll
-            for (int j = 0; j < V; ++j) {
-                if (hist) {
-                    const int k = j < nv ? count[c - c0 + j] : 0;
-                    if (k > 0) {
-                        v[j] = v[j] > 0.f ? v[j] / rep : v[j] * rep;
-                        const float f = freq * (float)k;
-                        v[j] = v[j] - f;
-                        v[j] = v[j] - pres;
-                    }
-                }
-                if (a.bias) v[j] = v[j] + b[j];
-                if (!((bits >> j) & 1u)) v[j] = -INFINITY;
+    for (int n = blockIdx.z; n < a.N; n += gridDim.z) {
+        float rep = 1.f, pres = 0.f, freq = 0.f;
+        if (hist) {
+            rep = a.repetition ? a.repetition[n] : a.all_repetition;
+            pres = a.presence ? a.presence[n] : a.all_presence;
+            freq = a.frequency ? a.frequency[n] : a.all_frequency;
+            for (int i = threadIdx.x; i < c1 - c0; i += 256) count[i] = 0;
+            __syncthreads();
+            const int L = seq_len(a.hist_lens, n, a.L);
+            const I* h = (const I*)a.history + n * a.hist_n;
+            for (int i = threadIdx.x; i < L; i += 256) {
+                const I c = h[i];
+                if (c >= c0 && c < c1) atomicAdd(&count[(int)(c - c0)], 1);
             }
-            store_vec<T, V>(out + c, nv, v);
+            __syncthreads();
         }
+        const int tx = threadIdx.x & ((1 << tx_bits) - 1), ty = threadIdx.x >> tx_bits;
+        const int t1 = min((int)(blockIdx.y + 1) * rows, a.T);
+        for (int t = blockIdx.y * rows + ty; t < t1; t += 256 >> tx_bits) {
+            const T* in = (const T*)a.logits + n * a.l_n + t * a.l_t;
+            T* out = (T*)a.out + n * a.o_n + t * a.o_t;
+            const unsigned* mask = a.mask ? a.mask + n * a.mask_n + t * a.mask_t : nullptr;
+            for (int c = c0 + tx * V; c < c1; c += V << tx_bits) {
+                const int nv = min(V, c1 - c);
+                float v[V], b[V];
+                load_vec<T, V>(in + c, nv, v);
+                const unsigned bits = mask ? mask[c >> 5] >> (c & 31) : ~0u;
+                if (a.bias) load_vec<float, V>(a.bias + n * a.bias_n + c, nv, b);
+#pragma unroll
+                for (int j = 0; j < V; ++j) {
+                    if (hist) {
+                        const int k = j < nv ? count[c - c0 + j] : 0;
+                        if (k > 0) {
+                            v[j] = v[j] > 0.f ? v[j] / rep : v[j] * rep;
+                            const float f = freq * (float)k;
+                            v[j] = v[j] - f;
+                            v[j] = v[j] - pres;
+                        }
+                    }
+                    if (a.bias) v[j] = v[j] + b[j];
+                    if (!((bits >> j) & 1u)) v[j] = -INFINITY;
+                }
+                store_vec<T, V>(out + c, nv, v);
+            }
+        }
+        if (hist) __syncthreads();            // the counters are the next line's
     }
 }
 
@@ -73,8 +76,8 @@ int launch(const krk_constrain_args& a, hipStream_t s) {
     int rows = 256 >> bits;
     while ((long)a.N * chunks * ((a.T + rows - 1) / rows) > 4096 && rows < a.T) rows *= 2;
     const int parts = (a.T + rows - 1) / rows;
-    if (a.N > 65535 || parts > 65535) return -4;
-    hipLaunchKernelGGL((constrain_kernel<T, I>), dim3(chunks, parts, a.N), dim3(256), 0, s, a, bits, rows);
+    if (parts > 65535) return -4;
+    hipLaunchKernelGGL((constrain_kernel<T, I>), dim3(chunks, parts, min(a.N, 65535)), dim3(256), 0, s, a, bits, rows);
     return hipGetLastError() == hipSuccess ? 0 : -1;
 }
 

@@ -46,7 +46,7 @@ def test_c_entries_refuse_null():
 
 
 @pytest.mark.parametrize('bad,code', [(dict(x=None), -1), (dict(y=None), -1), (dict(D=0), -1), (dict(N=-1), -1), (dict(T=-1), -1), (dict(type=3), -1),
-                                      (dict(K=0), -4), (dict(K=9), -4), (dict(state=PTR, state_out=PTR), -1)])
+                                      (dict(K=0), -4), (dict(K=9), -4), (dict(T=2 ** 30 + 1), -4), (dict(state=PTR, state_out=PTR), -1)])
 def test_c_conv_refusals(bad, code):
     assert conv(**bad) == code
     assert b'krk_causal_conv' in _lib.load().krk_last_error()
@@ -62,7 +62,7 @@ def test_c_scan_refusals(bad, code):
 
 
 @pytest.mark.parametrize('bad,code', [(dict(k=None), -1), (dict(H=3), -1), (dict(Hk=0), -1), (dict(E=257), -4), (dict(E=0), -4), (dict(Tq=-1), -1),
-                                      (dict(documents=PTR, Tq=3), -1), (dict(cap=-1.0), -1), (dict(cap=float('nan')), -1), (dict(type=7), -1)])
+                                      (dict(documents=PTR, Tq=3), -1), (dict(Tk=2 ** 30 + 1), -4), (dict(cap=-1.0), -1), (dict(cap=float('nan')), -1), (dict(type=7), -1)])
 def test_c_attention_refusals(bad, code):
     lib = _lib.load()
     assert lib.krk_attention(ctypes.byref(attention_args(**bad)), None) == code

@@ -411,10 +411,10 @@ def test_attention_rows_that_see_nothing_are_zero(dtype):
 
 @pytest.mark.parametrize('dtype', TYPES)
 @pytest.mark.parametrize('bad', [float('nan'), float('inf'), -float('inf')])
-def test_attention_what_may_not_be_seen_does_not_matter(dtype, bad):
+@pytest.mark.parametrize('t,e', [(150, 64), (300, 50), (150, 13), (300, 128), (150, 200), (150, 3)])
+def test_attention_what_may_not_be_seen_does_not_matter(dtype, bad, t, e):
     """Behind the valid keys, in other documents, and behind the query's position: whatever stands there."""
-    t = 150
-    q, k, v = qkv(2, t, t, 4, 2, 64, dtype)
+    q, k, v = qkv(2, t, t, 4, 2, e, dtype)
     ids = (torch.arange(t) // 47).int().expand(2, t).contiguous().to(DEV)
     lens = torch.tensor([t, 70])
     want = attention(q, k, v, lens, causal=True, documents=ids)
@@ -428,6 +428,51 @@ def test_attention_what_may_not_be_seen_does_not_matter(dtype, bad):
         same[at[0], (ids[at[0]] != ids[at]).cpu()] = True
         assert torch.equal(got[same.to(DEV)], want[same.to(DEV)]), at
         assert not got[at].isfinite().all()
+
+
+@pytest.mark.parametrize('dtype', TYPES)
+@pytest.mark.parametrize('e', [64, 37])
+def test_attention_one_odd_value(dtype, e):
+    """A single infinity among the values reaches its channel of the queries that see it, and nothing else."""
+    t = 140
+    q, k, v = qkv(1, t, t, 2, 1, e, dtype)
+    want = attention(q, k, v, causal=True)
+    for j, c, bad in ((0, 0, math.inf), (100, e - 1, -math.inf), (139, 5, math.nan), (63, 31, math.inf)):
+        v2 = v.clone()
+        v2[0, j, 0, c] = bad
+        got = attention(q, k, v2, causal=True)
+        hit = torch.zeros(1, t, 2, e, dtype=torch.bool, device=DEV)
+        hit[:, j:, :, c] = True
+        assert torch.equal(got[~hit], want[~hit])
+        assert got[hit].isnan().all() if bad != bad else (got[hit] == bad).all()
+    v2 = v.clone()
+    v2[0, 10, 0, 3], v2[0, 90, 0, 3] = math.inf, -math.inf
+    got = attention(q, k, v2, causal=True)
+    assert (got[0, 10:90, :, 3] == math.inf).all() and got[0, 90:, :, 3].isnan().all() and torch.equal(got[0, :10], want[0, :10])
+
+
+@pytest.mark.parametrize('dtype', TYPES)
+@pytest.mark.parametrize('scale', [0.0, -0.3, 2.0])
+@pytest.mark.parametrize('tq', [1, 70])
+def test_attention_scales(dtype, scale, tq):
+    q, k, v = qkv(2, tq, 70, 4, 2, 40, dtype)
+    got = attention(q, k, v, scale=scale)
+    want, bound = attention_ref(q, k, v, scale=scale)
+    check(got, want, bound)
+
+
+def test_attention_large_scores():
+    """Scores of thousands: one key takes all, and growing ones move the reference point again and again."""
+    t = 200
+    q = torch.ones(1, t, 1, 64, device=DEV)
+    k = (torch.arange(t, device=DEV).float() - 100)[None, :, None, None].expand(1, t, 1, 64).contiguous()
+    v = rand(1, t, 1, 64)
+    got = attention(q, k, v, causal=True)                              # scores 8 (j - 100): the next one is e^-8 of the last
+    want, bound = attention_ref(q, k, v, causal=True)
+    check(got, want, bound)
+    # the reference point is a rounded score, so the one weight p is 2^(its rounding), not 1: fl(fl(p v) fl(1 / p)) is v within three roundings
+    got = attention(q, k.flip(1) * 40, v)[0, 0]
+    assert ((got - v[0, 0]).abs() <= 3 * U * 1.001 * v[0, 0].abs()).all()
 
 
 def test_attention_strides():
@@ -578,6 +623,14 @@ def test_constrain_logits_broadcast_and_strides():
     big[:, 2:8, 11:111] = 5.0
     assert (big == 5).all()
     assert torch.equal(constrain_logits(x.transpose(1, 2).contiguous().transpose(1, 2), mask=mask), want)
+
+
+def test_constrain_logits_many_lines():
+    x = rand(70000, 9)
+    h = torch.randint(0, 9, (70000, 4), generator=torch.Generator().manual_seed(1)).to(DEV)
+    got = constrain_logits(x, history=h, presence=0.5)
+    hit = torch.zeros(70000, 9, dtype=torch.bool, device=DEV).scatter_(1, h, True)
+    assert torch.equal(got, torch.where(hit, x - 0.5, x))
 
 
 def test_constrain_logits_nothing_to_do():
