@@ -70,20 +70,17 @@ def constrain_logits(logits: torch.Tensor, *, mask: Optional[torch.Tensor] = Non
     shape = getattr(logits, 'shape', ())
     step = isinstance(logits, torch.Tensor) and logits.dim() == 2
     x = _first(logits, 'logits', 2 if step else 3)
-    if step:
-        x = x.unsqueeze(1)
-    n, t, c = x.shape
+    n, t, c = (shape[0], 1, shape[1]) if step else shape
     words = (c + 31) // 32
     if bias is not None:
         bias = _like(bias, 'bias', (c,) if isinstance(bias, torch.Tensor) and bias.dim() == 1 else (n, c), x, torch.float32)
     mn = mt = 0
     if mask is not None:
-        m = mask.unsqueeze(1) if isinstance(mask, torch.Tensor) and mask.dim() == 2 else mask
-        lead = tuple(getattr(m, 'shape', ()))[:2]
-        if lead not in ((n, 1), (1, 1), (n, t), (1, t)):
+        lead = tuple(getattr(mask, 'shape', ()))[:-1]
+        if len(lead) not in (1, 2) or lead[0] not in (n, 1) or lead[1:] not in ((), (1,), (t,)):
             raise ValueError(f'mask has to be (lines or 1, words) or (lines or 1, steps, words), got {tuple(getattr(mask, "shape", ()))}')
-        mask = _like(m, 'mask', (*lead, words), x, torch.int32)
-        mn, mt = (mask.stride(0) if lead[0] > 1 else 0), (mask.stride(1) if lead[1] > 1 else 0)
+        mask = _like(mask, 'mask', (*lead, words), x, torch.int32)
+        mn, mt = (mask.stride(0) if lead[0] > 1 else 0), (mask.stride(1) if len(lead) == 2 and lead[1] > 1 else 0)
     length, lens, wide = 0, None, 0
     rep, pres, freq = (_penalty(p, s, n, x, s == 'repetition') for p, s in
                        ((repetition, 'repetition'), (presence, 'presence'), (frequency, 'frequency')))
@@ -98,19 +95,17 @@ def constrain_logits(logits: torch.Tensor, *, mask: Optional[torch.Tensor] = Non
     elif history_lens is not None:
         raise ValueError('history_lens without history')
     if out is None:
-        y = x.new_empty(x.shape)
-        result = y.squeeze(1) if step else y
+        out = x.new_empty(x.shape)
     else:
         if _like(out, 'out', shape, x) is not out:
             raise ValueError('out is written in place: its classes have to be adjacent')
-        result, y = out, out.unsqueeze(1) if step else out
-        same = y.data_ptr() == x.data_ptr() and all(i == j or s == 1 for i, j, s in zip(y.stride(), x.stride(), x.shape))
-        _own_memory(y, 'out', (None if same else x, mask, bias, history, lens, rep[0], pres[0], freq[0]))
+        same = out.data_ptr() == x.data_ptr() and all(i == j or s == 1 for i, j, s in zip(out.stride(), x.stride(), x.shape))
+        _own_memory(out, 'out', (None if same else x, mask, bias, history, lens, rep[0], pres[0], freq[0]))
     if n == 0 or t == 0 or c == 0:
-        return result
-    a = _lib.KrkConstrainArgs(x.data_ptr(), y.data_ptr(), _ptr(mask), _ptr(bias), _ptr(history), _ptr(lens), _ptr(rep[0]), _ptr(pres[0]),
-                              _ptr(freq[0]), x.stride(0), x.stride(1), y.stride(0), y.stride(1), mn, mt,
+        return out
+    a = _lib.KrkConstrainArgs(x.data_ptr(), out.data_ptr(), _ptr(mask), _ptr(bias), _ptr(history), _ptr(lens), _ptr(rep[0]), _ptr(pres[0]),
+                              _ptr(freq[0]), x.stride(0), 0 if step else x.stride(1), out.stride(0), 0 if step else out.stride(1), mn, mt,
                               bias.stride(0) if bias is not None and bias.dim() == 2 else 0, history.stride(0) if history is not None else 0,
                               n, t, c, length, _TYPES[x.dtype], wide, rep[1], pres[1], freq[1])
     _call(_lib.load().krk_constrain_logits, a, x.device)
-    return result
+    return out

@@ -83,6 +83,13 @@ def _lengths(lens, name, n, top, dev):
     return lens.to(device=dev, dtype=torch.int32)
 
 
+def _extent(t):
+    """Bytes from a tensor's first element to behind its last one."""
+    if t.is_contiguous():
+        return t.nbytes
+    return (1 + sum((sz - 1) * st for st, sz in zip(t.stride(), t.shape))) * t.element_size() if t.numel() else 0
+
+
 def _own_memory(t, name, others):
     """A tensor that a call updates in place: no element twice, and nothing shared with the inputs."""
     end = t.numel()
@@ -95,7 +102,7 @@ def _own_memory(t, name, others):
     lo = t.data_ptr()
     hi = lo + end * t.element_size()
     for o in others:
-        if o is not None and o.data_ptr() < hi and lo < o.data_ptr() + o.nbytes:
+        if o is not None and o.data_ptr() < hi and lo < o.data_ptr() + _extent(o):
             raise ValueError(f'{name} shares memory with another argument: it is updated in place')
 
 
@@ -292,6 +299,24 @@ def _finite(v, name, least):
     return v
 
 
+def _keys(q, n, h, e, k, v):
+    if not isinstance(k, torch.Tensor) or k.dim() != 4:
+        raise ValueError('k has to be (N, Tk, Hk, E)')
+    tk, hk = k.shape[1], k.shape[2]
+    k, v = _like(k, 'k', (n, tk, hk, e), q), _like(v, 'v', (n, tk, hk, e), q)
+    if h == 0 or hk == 0 or h % hk:
+        raise ValueError(f'{hk} key heads have to divide {h} query heads')
+    if not 1 <= e <= 256:
+        raise ValueError(f'heads of {e} channels: 1 to 256 are supported')
+    return k, v, tk, hk
+
+
+def _scores(q, h, e, slopes, cap, scale):
+    if slopes is not None:
+        slopes = _like(slopes, 'slopes', (h,), q, torch.float32)
+    return slopes, _finite(cap, 'cap', 0), e ** -0.5 if scale is None else _finite(scale, 'scale', -math.inf)
+
+
 def attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, seq_lens: Lens = None, *, key_lens: Lens = None, causal: bool = False,
               align: str = 'start', prefix_lens: Lens = None, documents: Optional[torch.Tensor] = None, slopes: Optional[torch.Tensor] = None,
               cap: float = 0.0, scale: Optional[float] = None) -> torch.Tensor:
@@ -308,14 +333,7 @@ def attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, seq_lens: Lens 
     """
     q = _first(q, 'q', 4)
     n, tq, h, e = q.shape
-    if not isinstance(k, torch.Tensor) or k.dim() != 4:
-        raise ValueError('k has to be (N, Tk, Hk, E)')
-    tk, hk = k.shape[1], k.shape[2]
-    k, v = _like(k, 'k', (n, tk, hk, e), q), _like(v, 'v', (n, tk, hk, e), q)
-    if h == 0 or hk == 0 or h % hk:
-        raise ValueError(f'{hk} key heads have to divide {h} query heads')
-    if not 1 <= e <= 256:
-        raise ValueError(f'heads of {e} channels: 1 to 256 are supported')
+    k, v, tk, hk = _keys(q, n, h, e, k, v)
     if align not in ('start', 'end'):
         raise ValueError(f"align has to be 'start' or 'end', not {align!r}")
     dev = q.device
@@ -328,21 +346,28 @@ def attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, seq_lens: Lens 
         if tq != tk:
             raise ValueError('documents need as many queries as keys')
         documents = _like(documents, 'documents', (n, tq), q, torch.int32)
-    if slopes is not None:
-        slopes = _like(slopes, 'slopes', (h,), q, torch.float32)
-    cap, scale = _finite(cap, 'cap', 0), e ** -0.5 if scale is None else _finite(scale, 'scale', -math.inf)
-    out = q.new_empty((n, tq, h, e))
+    slopes, cap, scale = _scores(q, h, e, slopes, cap, scale)
+    return _attend(q, (n, tq, h, e), k, v, tk, hk, q_lens, k_lens, prefix, documents, slopes, bool(causal), align == 'end', scale, cap)
+
+
+def _attend(q, shape, k, v, tk, hk, q_lens, k_lens, prefix, documents, slopes, causal, at_end, scale, cap):
+    """The call itself, its arguments checked: q (N, Tq, H, E), or (N, H, E) for one step."""
+    n, tq, h, e = shape
+    out = q.new_empty(q.shape)
     if n == 0 or tq == 0:
         return out
     if tk == 0:
         return out.zero_()
+    if q.dim() == 4:
+        qs, os = q.stride()[:3], (tq * h * e, h * e, e)
+    else:
+        qs, os = (q.stride(0), 0, q.stride(1)), (h * e, 0, e)
     a = _lib.KrkAttentionArgs(q.data_ptr(), k.data_ptr(), v.data_ptr(), out.data_ptr(), _ptr(q_lens), _ptr(k_lens), _ptr(prefix), _ptr(documents),
-                              _ptr(slopes), None, 0, *q.stride()[:3], *k.stride()[:3], *v.stride()[:3], *out.stride()[:3],
-                              documents.stride(0) if documents is not None else 0, n, tq, tk, h, hk, e, _TYPES[q.dtype], bool(causal),
-                              align == 'end', scale, cap)
+                              _ptr(slopes), None, 0, *qs, *k.stride()[:3], *v.stride()[:3], *os,
+                              documents.stride(0) if documents is not None else 0, n, tq, tk, h, hk, e, _TYPES[q.dtype], causal, at_end, scale, cap)
     lib = _lib.load()
-    scratch = _scratch(lib.krk_attention_workspace, a, dev)                 # noqa: F841 (alive until the launch is enqueued)
-    _call(lib.krk_attention, a, dev)
+    scratch = _scratch(lib.krk_attention_workspace, a, q.device)            # noqa: F841 (alive until the launch is enqueued)
+    _call(lib.krk_attention, a, q.device)
     return out
 
 
@@ -353,4 +378,8 @@ def attention_step(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor
     last of which is the step's own.  The caches may be strided views of larger ones.  Returns (N, H, E); zeros for an empty cache.
     """
     q = _first(q, 'q', 3)
-    return attention(q.unsqueeze(1), k_cache, v_cache, key_lens=cache_lens, align='end', slopes=slopes, cap=cap, scale=scale).squeeze(1)
+    n, h, e = q.shape
+    k, v, tk, hk = _keys(q, n, h, e, k_cache, v_cache)
+    lens = _lengths(cache_lens, 'cache_lens', n, tk, q.device)
+    slopes, cap, scale = _scores(q, h, e, slopes, cap, scale)
+    return _attend(q, (n, 1, h, e), k, v, tk, hk, None, lens, None, None, slopes, False, True, scale, cap)

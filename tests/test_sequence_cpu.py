@@ -116,6 +116,8 @@ def test_tensors_that_are_updated_in_place():
             sequence._own_memory(bad, 'state', ())
     with pytest.raises(ValueError):
         sequence._own_memory(t[2], 'state', (None, t[1:3]))
+    with pytest.raises(ValueError):
+        sequence._own_memory(t[4], 'state', (t[::4, :1, :1],))           # few elements, far apart
     sequence._own_memory(t[2], 'state', (t[:2], t[3:], torch.zeros(4)))
 
 
