@@ -19,14 +19,19 @@ __global__ __launch_bounds__(256) void conv_seq_kernel(krk_conv_args a, int grou
     const int run = id / groups, d0 = (id - run * groups) * V;
     if (run >= runs) return;
     const int nv = min(V, a.D - d0);
-    float w[K][V], b[V];
+    // the kernels of V neighbouring channels lie behind one another: K vectors, put in order in the registers
+    float w[K][V], b[V], flat[K * V];
 #pragma unroll
-    for (int j = 0; j < V; ++j) {
-        const int d = d0 + (j < nv ? j : 0);
+    for (int k = 0; k < K; ++k)
+        load_vec<T, V>((const T*)a.weight + (long)d0 * K + k * V, nv * K - k * V, *reinterpret_cast<float (*)[V]>(&flat[k * V]));
 #pragma unroll
-        for (int k = 0; k < K; ++k) w[k][j] = to_f<T>(((const T*)a.weight)[(long)d * K + k]);
-        b[j] = a.bias ? to_f<T>(((const T*)a.bias)[d]) : 0.f;
-    }
+    for (int j = 0; j < V; ++j)
+#pragma unroll
+        for (int k = 0; k < K; ++k) w[k][j] = flat[j * K + k];
+    if (a.bias) load_vec<T, V>((const T*)a.bias + d0, nv, b);
+    else
+#pragma unroll
+        for (int j = 0; j < V; ++j) b[j] = 0.f;
     for (int n = blockIdx.y; n < a.N; n += gridDim.y) {
         const int len = seq_len(a.lens, n, a.T);
         const T* x = (const T*)a.x + n * a.x_n + d0;

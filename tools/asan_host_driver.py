@@ -104,6 +104,31 @@ for spec in specs:
             plan.close(); twin.close()
         else:
             twin.close(); plan.close()
+# the operators on sequence rows: their argument checks, workspace sizes and launch shapes over the whole range of sizes
+any_size = lambda hi: int(2 ** rng.uniform(0, np.log2(hi)))  # noqa: E731
+for _ in range(400):
+    kind, AT = int(rng.integers(3)), 4096               # AT stands for an address: launches are no-ops, the host reads none of it
+    conv = _lib.KrkConvArgs(x=AT, weight=AT, y=AT, state_out=2 * AT, N=any_size(1 << 20), T=any_size(1 << 20), D=any_size(1 << 14),
+                            K=int(rng.integers(0, 10)), type=kind)
+    g = int(rng.integers(1, 4))
+    scan = _lib.KrkScanArgs(x=AT, dt=AT, A=AT, B=AT, C=AT, y=AT, N=any_size(1 << 18), T=any_size(1 << 20), D=g * any_size(1 << 13),
+                            S=any_size(300), G=g, type=kind)
+    hk = any_size(16)
+    attn = _lib.KrkAttentionArgs(q=AT, k=AT, v=AT, out=AT, N=any_size(1 << 12), Tq=any_size(1 << 16), Tk=any_size(1 << 20), H=hk * any_size(8), Hk=hk,
+                                 E=any_size(300), type=kind, scale=1.0, causal=int(rng.integers(2)))
+    if rng.integers(2):
+        attn.Tk, attn.documents = attn.Tq, AT
+    cons = _lib.KrkConstrainArgs(logits=AT, out=AT, history=AT, L=any_size(1 << 14), N=any_size(1 << 18), T=any_size(1 << 12), C=any_size(1 << 20), type=kind)
+    for args, run, size in ((conv, lib.krk_causal_conv, None), (scan, lib.krk_selective_scan, lib.krk_selective_scan_workspace),
+                            (attn, lib.krk_attention, lib.krk_attention_workspace), (cons, lib.krk_constrain_logits, None)):
+        need = size(C.byref(args)) if size else 0
+        if need > 0:
+            args.workspace, args.workspace_bytes = AT, need - 1
+            assert run(C.byref(args), None) == _lib.KRK_E_INVALID
+            args.workspace_bytes = need
+        rc = run(C.byref(args), None)
+        assert rc in (_lib.KRK_OK, _lib.KRK_E_UNSUPPORTED), (rc, lib.krk_last_error())
+        calls += 1
 live = fake.fake_hip_live_allocations()
 assert live == 0, f'{live} device allocations were never freed'
 print(f'ASAN-HOST OK {plans} plans ({skipped} specs refused at construction), {calls} calls, {fake.fake_hip_launches()} launches')
