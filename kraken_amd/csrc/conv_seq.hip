@@ -3,8 +3,10 @@
 //   p_i = bias + sum_k w[d][k] x_{i-(K-1)+k}[d],   y = p or p sigmoid(p),   i in processing order over the valid steps of a row
 //
 // 2 K flops per element read and written: bound by memory.  A thread owns one 16-byte channel group and walks a run of steps with the
-// last K-1 inputs in registers, so every input is read once (plus K-1 of them again per run); U steps' loads are issued before any of them
-// is used.  Lanes of a wave lie along the channels, so a wave's access is contiguous.
+// last K-1 inputs in registers, so every input is read once (plus K-1 of them again per run); the next U steps' loads are in flight while U
+// steps are computed.  Lanes of a wave lie along the channels, so a wave's access is contiguous.
+// 2 x 16384 x 4096 bf16, K = 4: 110 us = 4.9 TB/s, the rate of a copy (without the loads in flight 137 us; U = 8: the same, and fp32 lines a fifth
+// slower); 256 ragged lines of 150 x 400 fp32: 23 us.  One step of 8 x 800 channels: 6 us, the latency of its two dependent loads.
 #include "seq.h"
 
 namespace {
