@@ -8,10 +8,10 @@
 //
 // What bounds it: 16-bit heads of 64 channels the vector units (per score a multiply-add, an exponential, a maximum, a sum and half a conversion
 // against 16 matrix instructions per 64 x 32 scores; the cap adds an exponential and a reciprocal): 2 x 4000 x 16 x 64 fp16, capped, causal with a prefix:
-// 164 us, 330 TFLOP/s.  fp32 the matrix units on long rows (16 x 2048 x 8 x 64: 118 of 154 TFLOP/s), on short lines the loads in front of each
-// workgroup, which two waves per SIMD do not cover (256 ragged lines of 150 x 8 x 50: 132 us, 46 of them matrix time).  Packed documents
+// 158 us, 342 TFLOP/s.  fp32 the matrix units on long rows (16 x 2048 x 8 x 64: 118 of 154 TFLOP/s), on short lines the loads in front of each
+// workgroup, which two waves per SIMD do not cover (256 ragged lines of 150 x 8 x 50: 131 us, 46 of them matrix time).  Packed documents
 // (8192 steps, 24 of them, 16 x 128 bf16): 72 + 5 us, most of it the latency of 1 to 16 tiles per workgroup.
-// 128 queries a workgroup where rows are long: keys are read from the L2 half as often; 64 on short lines (133 against 200 us for the lines above).
+// 128 queries a workgroup where rows are long: keys are read from the L2 half as often; 64 on short lines (131 against 200 us for the lines above).
 #include "attn_seq.h"
 
 namespace {
@@ -241,13 +241,16 @@ __global__ __launch_bounds__(NW * 64, EP * sizeof(T) > 256 ? 1 : 2) void attn_ti
     // in part can do that; they are searched while they go to LDS.
     auto search = [&](int t) { return docs || (t + 1) * BK > bmin; };
     auto put = [&](int t, int buf, int turn) {
-        unsigned high = 0;
+        bool hit = false;
+        if (search(t)) {
+            unsigned high = 0;
 #pragma unroll
-        for (int x = 0; x < CPT; ++x)
+            for (int x = 0; x < CPT; ++x)
 #pragma unroll
-            for (int i = 0; i < 4; ++i) high = odd_max<T>(high, vr[x][i]);
-        const bool hit = search(t) && odd_found<T>(high);
-        if (hit) odd[turn & 3] = 1;
+                for (int i = 0; i < 4; ++i) high = odd_max<T>(high, vr[x][i]);
+            hit = odd_found<T>(high);
+            if (hit) odd[turn & 3] = 1;
+        }
 #pragma unroll
         for (int x = 0; x < CPT; ++x) {
             const int id = threadIdx.x + x * NT, row = id / CPR, e = (id - row * CPR) * CV;
