@@ -258,7 +258,7 @@ int launch_rows(const krk_attention_args& a, hipStream_t s) {
     const int rep = a.H / a.Hk, blocks_h = (rep + R - 1) / R, splits = split_count(a);
     int span = (a.Tk + splits - 1) / splits;
     const long items = (long)a.N * a.Tq * a.Hk * blocks_h, rows = (long)a.N * a.Tq * a.H;
-    if (items > 0x7fffff00L) return -4;
+    if (seq_grid_too_large(items, 256)) return -4;
     hipLaunchKernelGGL((attn_rows_kernel<T, R, LE>), dim3((unsigned)items, splits), dim3(256), 0, s, a, blocks_h, splits, span);
     if (splits > 1) hipLaunchKernelGGL((attn_join_kernel<T>), dim3((unsigned)((rows + 3) / 4)), dim3(256), 0, s, a, splits, rows);
     return hipGetLastError() == hipSuccess ? 0 : -1;

@@ -485,7 +485,7 @@ int launch(const krk_attention_args& a, const AttnTiles& g, void* scratch, hipSt
     const int qblocks = (a.Tq + NW * 32 - 1) / (NW * 32), tiles = (a.Tk + g.keys - 1) / g.keys;
     const int2* ranges = nullptr;
     if (a.documents) {
-        if ((long)a.N * tiles > 0x7fffff00L) return -4;
+        if (seq_grid_too_large((long)a.N * tiles, 64)) return -4;
         int2* r = (int2*)scratch;
         ranges = r;
         hipLaunchKernelGGL(attn_ranges_kernel, dim3((unsigned)(((long)a.N * tiles + 3) / 4)), dim3(256), 0, s, a, r, tiles, g.keys);
@@ -495,7 +495,7 @@ int launch(const krk_attention_args& a, const AttnTiles& g, void* scratch, hipSt
     // only causal rows differ in length by their place; elsewhere one key head at a time is better for the L2 (lines: 138 against 143 us)
     const int batch = !a.causal || a.documents ? 1 : (int)max(1L, min(64L, (4L << 20) / (2L * a.Tk * a.E * (long)sizeof(T) / cut + 1)));
     const long blocks = groups * cut * ((qblocks * (long)(a.H / a.Hk) + cut - 1) / cut);
-    if (blocks > 0x7fffff00L) return -4;
+    if (seq_grid_too_large(blocks, NW * 64)) return -4;
     hipLaunchKernelGGL((attn_tile_kernel<T, EP, NW>), dim3((unsigned)blocks, g.splits), dim3(NW * 64), 0, s, a, qblocks, cut, batch, g.splits, tiles, ranges);
     return hipGetLastError() == hipSuccess ? 0 : -1;
 }

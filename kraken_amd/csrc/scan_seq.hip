@@ -246,7 +246,7 @@ int launch(const krk_scan_args& a, hipStream_t s) {
     const int per_block = 256 / LP;
     const long blocks = (long)a.G * ((a.D / a.G + per_block - 1) / per_block);
     const unsigned rows = (unsigned)min(a.N, 65535);
-    if (blocks > 0x7fffff00L) return -4;
+    if (seq_grid_too_large(blocks, 256)) return -4;
     if (c.chunks > 1) {
         hipLaunchKernelGGL((scan_seq_kernel<T, LP, SL, false>), dim3((unsigned)blocks, c.chunks - 1, rows), dim3(256), 0, s, a, c);
         hipLaunchKernelGGL(scan_join_kernel, dim3((unsigned)(((long)a.D * a.S + 255) / 256), rows), dim3(256), 0, s, a, c);
@@ -258,7 +258,7 @@ int launch(const krk_scan_args& a, hipStream_t s) {
 template <class T, int LP>
 int launch_step(const krk_scan_args& a, hipStream_t s) {
     const long blocks = ((long)a.N * a.D * LP + 255) / 256;
-    if (blocks > 0x7fffff00L) return -4;
+    if (seq_grid_too_large(blocks, 256)) return -4;
     hipLaunchKernelGGL((scan_step_kernel<T, LP>), dim3((unsigned)blocks), dim3(256), 0, s, a);
     return hipGetLastError() == hipSuccess ? 0 : -1;
 }

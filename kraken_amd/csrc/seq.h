@@ -73,7 +73,10 @@ __device__ __forceinline__ int seq_len(const int* lens, int n, int T) {
     return lens ? min(max(lens[n], 0), T) : T;
 }
 
-// launchers: 0, or -1 when the launch failed
+// a grid's threads fit 32 bits
+inline bool seq_grid_too_large(long blocks, int threads) { return blocks > 0xffffffffL / threads; }
+
+// launchers: 0, -1 when the launch failed, -4 for more rows than a grid holds
 int krk_launch_causal_conv(const krk_conv_args& a, hipStream_t s);
 long krk_scan_workspace(const krk_scan_args& a);
 int krk_launch_selective_scan(const krk_scan_args& a, hipStream_t s);
