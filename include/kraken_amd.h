@@ -50,7 +50,7 @@
 extern "C" {
 #endif
 
-#define KRK_ABI_VERSION 4   /* 4: + the sequence operators and krk_constrain_logits; 3 (round 6): + krk_plan_clone; 2 (round 6): + krk_plan_get_recurrence; round 5 had added CONVT / RESHAPE ops, krk_plan_out_dims, krk_plan_olens_w, krk_plan_set_recurrence under version 1 */
+#define KRK_ABI_VERSION 4   /* 4: + the sequence operators and krk_constrain_logits; 3: + krk_plan_clone; 2: + krk_plan_get_recurrence, on top of the CONVT / RESHAPE ops, krk_plan_out_dims, krk_plan_olens_w and krk_plan_set_recurrence */
 
 /* error codes */
 #define KRK_OK            0
