@@ -76,7 +76,7 @@ def _lengths(lens, name, n, top, dev):
             lens = lens.clamp(0, top).int()
         return lens.contiguous()
     lens = torch.as_tensor(lens)
-    if lens.shape != (n,) or lens.is_floating_point() or lens.dtype == torch.bool:
+    if lens.shape != (n,) or (n and (lens.is_floating_point() or lens.dtype == torch.bool)):
         raise ValueError(f'{name} needs one whole number per line')
     if n and (int(lens.min()) < 0 or int(lens.max()) > top):
         raise ValueError(f'{name} outside [0, {top}]')

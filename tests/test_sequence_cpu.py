@@ -149,3 +149,13 @@ def test_label_mask():
     for bad in ([-1], [40]):
         with pytest.raises(ValueError):
             constraints.label_mask([bad], 40, device='cpu')
+
+
+def test_lengths_of_an_empty_batch():
+    """An empty list has no whole numbers that its type could show: a batch of no lines takes it."""
+    got = sequence._lengths([], 'seq_lens', 0, 5, torch.device('cpu'))
+    assert got.shape == (0,) and got.dtype == torch.int32
+    with pytest.raises(ValueError, match='whole number'):
+        sequence._lengths([], 'seq_lens', 1, 5, torch.device('cpu'))
+    with pytest.raises(ValueError, match='whole number'):
+        sequence._lengths([1.0], 'seq_lens', 1, 5, torch.device('cpu'))
