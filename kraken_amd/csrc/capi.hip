@@ -2714,6 +2714,8 @@ static int attention_args_ok(const krk_attention_args* a) {
     if (seq_large({a->N, a->Tq, a->Tk, a->H})) return fail(KRK_E_UNSUPPORTED, "krk_attention: axes up to 2^30");
     if (a->documents && a->Tq != a->Tk) return fail(KRK_E_INVALID, "krk_attention: documents need as many queries as keys");
     if (!(a->cap >= 0.f)) return fail(KRK_E_INVALID, "krk_attention: cap must not be negative");
+    if (a->cap > 0.f && !std::isnormal(a->cap)) return fail(KRK_E_INVALID, "krk_attention: cap must be 0 or a normal number");
+    if (!std::isfinite(a->scale)) return fail(KRK_E_INVALID, "krk_attention: scale must be finite");
     return KRK_OK;
 }
 

@@ -293,7 +293,7 @@ def _scratch(fn, args, dev):
 
 # -------------------------------------------------------------------------------------------------------------------- attention
 def _finite(v, name, least):
-    v = float(v)
+    v = C.c_float(v).value                          # what the kernel gets: 1e39 is infinite there
     if not math.isfinite(v) or v < least:
         raise ValueError(f'{name} has to be finite{" and not negative" if least == 0 else ""}, got {v}')
     return v
@@ -314,6 +314,8 @@ def _keys(q, n, h, e, k, v):
 def _scores(q, h, e, slopes, cap, scale):
     if slopes is not None:
         slopes = _like(slopes, 'slopes', (h,), q, torch.float32)
+    if 0 < cap < 2.0 ** -126:
+        raise ValueError(f'cap has to be 0 or a normal float32, got {cap}')
     return slopes, _finite(cap, 'cap', 0), e ** -0.5 if scale is None else _finite(scale, 'scale', -math.inf)
 
 

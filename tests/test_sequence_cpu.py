@@ -159,3 +159,24 @@ def test_lengths_of_an_empty_batch():
         sequence._lengths([], 'seq_lens', 1, 5, torch.device('cpu'))
     with pytest.raises(ValueError, match='whole number'):
         sequence._lengths([1.0], 'seq_lens', 1, 5, torch.device('cpu'))
+
+
+@pytest.mark.parametrize('value,least', [(1e39, 0), (-1e39, -float('inf')), (float('nan'), 0), (-1.0, 0)])
+def test_numbers_that_float32_does_not_hold(value, least):
+    """The kernels take them as float32: 1e39 is infinite there."""
+    with pytest.raises(ValueError):
+        sequence._finite(value, 'scale', least)
+
+
+def test_caps_below_float32s_normal_range():
+    """1 / cap would be infinite, and a score of zero times it no number."""
+    for cap in (1e-39, 1e-60):
+        with pytest.raises(ValueError, match='cap'):
+            sequence._scores(None, 2, 4, None, cap, None)
+    assert sequence._scores(None, 2, 4, None, 1e-37, None)[1] > 0
+    assert sequence._scores(None, 2, 4, None, 0.0, None) == (None, 0.0, 0.5)
+
+
+@pytest.mark.parametrize('bad', [dict(cap=float('inf')), dict(cap=1e-39), dict(scale=float('inf')), dict(scale=float('nan'))])
+def test_c_attention_refuses_numbers_that_it_cannot_use(bad):
+    assert _lib.load().krk_attention(ctypes.byref(attention_args(**bad)), None) == _lib.KRK_E_INVALID
