@@ -5,6 +5,7 @@ Constraint of a network's scores in front of a decoder: the labels a line may ho
 kraken/lib/ctc_decoder.py:35-72, which takes the scores as they are): a form field that holds digits only, a page in one script, or the next
 label of a label model.  Like the decoder it has no CPU implementation: without a HIP device the call raises.
 """
+import ctypes as C
 from typing import Iterable, Optional, Union
 
 import numpy as np
@@ -45,7 +46,7 @@ def _penalty(p, name, n, first, positive=False):
     """(tensor or None, value): a number for all lines, or one per line."""
     if isinstance(p, torch.Tensor) and p.dim() == 1:
         return _like(p, name, (n,), first, torch.float32).contiguous(), 0.0
-    p = float(p)
+    p = C.c_float(float(p)).value                   # what the kernel gets: 1e-60 is zero there
     if not np.isfinite(p) or (positive and p <= 0):
         raise ValueError(f'{name} has to be finite{" and positive" if positive else ""}, got {p}')
     return None, p

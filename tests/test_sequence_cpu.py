@@ -180,3 +180,11 @@ def test_caps_below_float32s_normal_range():
 @pytest.mark.parametrize('bad', [dict(cap=float('inf')), dict(cap=1e-39), dict(scale=float('inf')), dict(scale=float('nan'))])
 def test_c_attention_refuses_numbers_that_it_cannot_use(bad):
     assert _lib.load().krk_attention(ctypes.byref(attention_args(**bad)), None) == _lib.KRK_E_INVALID
+
+
+def test_penalties_that_float32_does_not_hold():
+    """1e-60 is zero as float32, a divisor: the score would be infinite or no number."""
+    for value, positive in ((1e-60, True), (1e39, True), (1e39, False), (-1e39, False)):
+        with pytest.raises(ValueError):
+            constraints._penalty(value, 'penalty', 2, None, positive)
+    assert constraints._penalty(1.5, 'penalty', 2, None, True) == (None, 1.5)
