@@ -181,7 +181,7 @@ __global__ __launch_bounds__(256) void scan_join_kernel(krk_scan_args a, ScanCut
 #pragma unroll
             for (int c = 0; c < B; ++c)
                 if (c0 + c < cut.chunks - 1) {
-                    h = __builtin_fmaf(__builtin_amdgcn_exp2f(e[c] * A), h, q[c]);
+                    h = h == 0.f ? q[c] : __builtin_fmaf(__builtin_amdgcn_exp2f(e[c] * A), h, q[c]);   // growth over a chunk may be infinite
                     p[(c0 + c) * ds] = h;
                 }
         }

@@ -289,6 +289,15 @@ def test_selective_scan_step_sizes(s):
     check(st, want_after, bound_after)
 
 
+@pytest.mark.parametrize('t', [40, 900])
+def test_selective_scan_growth_from_nothing(t):
+    """A state of zero stays zero however large its factor: exp(10 * 17 steps) is infinite in fp32, and 0 times that no number."""
+    x = torch.zeros(1, t, 32, device=DEV)
+    A, bc = torch.full((32, 16), 10.0, device=DEV), torch.ones(1, t, 16, device=DEV)
+    y, state = selective_scan(x, torch.ones_like(x), A, bc, bc)
+    assert not y.any() and not state.any()
+
+
 def test_selective_scan_strides():
     c, k = scan_inputs(2, 70, 48, 16, 1, torch.float32, True)
     want, after = selective_scan(**c, **k, dt_softplus=True)
