@@ -31,15 +31,16 @@ __device__ __forceinline__ f32x16 mfma16(f16_t, const s16x8& a, const s16x8& b, 
 __device__ __forceinline__ f32x16 mfma16(float, const s16x8&, const s16x8&, const f32x16& c) { return c; }
 
 // A head is read in chunks of 16 bytes; where its E channels are no whole number of them, the last chunk is loaded so that it ENDS there: one load
-// without a condition whatever E is, and none past the row.  Its first channels are in the chunk before as well: keys and values are kept so,
-// the query has zeros in their place, and the result of such a channel is stored once.  Chunks behind the last repeat it, the query zero.
+// without a condition whatever E is, and none past the row.  Its first channels are in the chunk before as well: values are kept so,
+// the query and the keys have zeros in their place (both: 0 times an infinite key is no number), and the result of such a channel is stored once.
+// Chunks behind the last repeat it, query and key zero.
 template <class T> __device__ __forceinline__ u32x4 load_chunk(const T* row, int e, int E) {
     u32x4 r;
     __builtin_memcpy(&r, row + min(e, E - VecOf<T>::V), 16);
     return r;
 }
-// the query's chunk at e: without the channels that the chunk before has, and nothing behind the end
-template <class T> __device__ __forceinline__ u32x4 query_chunk(u32x4 r, int e, int E) {
+// the query's or a key's chunk at e: without the channels that the chunk before has, and nothing behind the end
+template <class T> __device__ __forceinline__ u32x4 own_chunk(u32x4 r, int e, int E) {
     typedef T Tv __attribute__((ext_vector_type(VecOf<T>::V)));
     Tv v = __builtin_bit_cast(Tv, r);
 #pragma unroll
@@ -240,8 +241,13 @@ __global__ __launch_bounds__(NW * 64, EP * sizeof(T) > 256 ? 1 : 2) void attn_ti
     // A value that is not finite must not reach the queries that may not see it: 0 x NaN is NaN.  Only tiles that some query of the workgroup sees
     // in part can do that; they are searched while they go to LDS.
     auto search = [&](int t) { return docs || (t + 1) * BK > bmin; };
+    constexpr bool ONE = NT % CPR == 0;                                   // a thread's chunks are all of the same channels
+    const u32x4 all = {~0u, ~0u, ~0u, ~0u}, keep = own_chunk<T>(all, (int)threadIdx.x % CPR * CV, a.E);
     auto put = [&](int t, int buf, int turn) {
         bool hit = false;
+        if (a.E != EP)
+#pragma unroll
+            for (int x = 0; x < CPT; ++x) kr[x] &= ONE ? keep : own_chunk<T>(all, (int)(threadIdx.x + x * NT) % CPR * CV, a.E);
         if (search(t)) {
             unsigned high = 0;
 #pragma unroll
@@ -281,7 +287,7 @@ __global__ __launch_bounds__(NW * 64, EP * sizeof(T) > 256 ? 1 : 2) void attn_ti
     if (tile >= 0) fetch(tile);
 #pragma unroll
     for (int x = 0; x < NQ; ++x) {
-        if (a.E != EP) raw[x] = query_chunk<T>(raw[x], STEP * x + STEP / 2 * half, a.E);
+        if (a.E != EP) raw[x] = own_chunk<T>(raw[x], STEP * x + STEP / 2 * half, a.E);
         if constexpr (F32) q32[x] = __builtin_bit_cast(f32x4, raw[x]) * sign;
         else {
             q16[x] = __builtin_bit_cast(s16x8, raw[x]);

@@ -470,6 +470,19 @@ def test_attention_scales(dtype, scale, tq):
     check(got, want, bound)
 
 
+@pytest.mark.parametrize('dtype', TYPES)
+@pytest.mark.parametrize('tq', [1, 70, 300])
+@pytest.mark.parametrize('e', [13, 50, 64, 100, 200])
+def test_attention_keys_of_minus_infinity(dtype, tq, e):
+    """Keys whose score is -inf have no weight: the result is the one without them, in any channel of a head."""
+    q, k, v = qkv(2, tq, 150, 4, 2, e, dtype, seed=6)
+    q = q.abs() + 0.125
+    kept = [j for j in range(150) if j not in (3, 70, 149)]
+    want, bound = attention_ref(q, k[:, kept], v[:, kept])
+    k[:, 3, :, e - 1] = k[:, 70, :, 0] = k[:, 149, :, max(0, e - 6)] = -math.inf
+    check(attention(q, k, v), want, bound, 'keys of -inf')
+
+
 def test_attention_large_scores():
     """Scores of thousands: one key takes all, and growing ones move the reference point again and again."""
     t = 200
