@@ -4,8 +4,11 @@
 
 constexpr float LOG2E = 1.4426950408889634f;
 
+// 16-bit results take cap tanh's error of 2^-23 of the cap up to this one (2^-13 of a weight then, a quarter of fp16's half step)
+constexpr float COARSE_CAP = 1024.f;
+
 // cap tanh(s / cap).  fp32: the odd series below 0.45 (the rest is under 2^-25 of it), where 1 - 2 / (1 + e^2x) would cancel; 16-bit results
-// need no more than the latter.
+// need no more than the latter up to COARSE_CAP.
 template <class T> __device__ __forceinline__ float seq_cap(float s, float cap, float rcap) {
     const float x = s * rcap, ax = fabsf(x);
     const float e = __builtin_amdgcn_exp2f(-2.f * LOG2E * ax);

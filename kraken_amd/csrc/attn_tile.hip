@@ -348,9 +348,9 @@ __global__ __launch_bounds__(NW * 64, EP * sizeof(T) > 256 ? 1 : 2) void attn_ti
                 if (!plain) {
                     scale = 1.f;
                     if (a.cap > 0.f) {
-                        if constexpr (F32) {
+                        if (F32 || a.cap > COARSE_CAP) {
                             const float raw = c * (1.f / LOG2E);
-                            EACH(s[x][i] = seq_cap<T>(s[x][i] * raw, a.cap, rcap) * LOG2E);
+                            EACH(s[x][i] = seq_cap<float>(s[x][i] * raw, a.cap, rcap) * LOG2E);
                         } else {                                          // cap tanh(x) = cap - 2 cap / (1 + e^2x): 2^-23 of cap off at most
                             const float cl = a.cap * LOG2E, cx = 2.f * c * rcap;
                             EACH(s[x][i] = __builtin_fmaf(-2.f * cl, __builtin_amdgcn_rcpf(1.f + __builtin_amdgcn_exp2f(s[x][i] * cx)), cl));

@@ -471,6 +471,16 @@ def test_attention_scales(dtype, scale, tq):
 
 
 @pytest.mark.parametrize('dtype', TYPES)
+@pytest.mark.parametrize('tq', [1, 70])
+def test_attention_cap_far_above_the_scores(dtype, tq):
+    """cap tanh(s / cap) = s (1 - (s / cap)^2 / 3 + ...): at 1e7 the scores themselves.  Eleven roundings of a score behind its product (two of the
+    scale, two of 1 / log2 e, the product with both, 1 / cap and the product with it, the polynomial, cap, two of log2 e) are three more than the
+    bound's E + 8 have: 3 x 40 steps at the sizes here, well within its 8 x 88, of which scores below 10 take 8 x 10."""
+    q, k, v = qkv(2, tq, 200, 4, 2, 48, dtype, seed=5)
+    check(attention(q, k, v, cap=1e7), *attention_ref(q, k, v), 'a cap that does nothing')
+
+
+@pytest.mark.parametrize('dtype', TYPES)
 @pytest.mark.parametrize('tq', [1, 70, 300])
 @pytest.mark.parametrize('e', [13, 50, 64, 100, 200])
 def test_attention_keys_of_minus_infinity(dtype, tq, e):
