@@ -8,10 +8,10 @@
 //
 // What bounds it: 16-bit heads of 64 channels the vector units (per score a multiply-add, an exponential, a maximum, a sum and half a conversion
 // against 16 matrix instructions per 64 x 32 scores; the cap adds an exponential and a reciprocal): 2 x 4000 x 16 x 64 fp16, capped, causal with a prefix:
-// 158 us, 342 TFLOP/s.  fp32 the matrix units on long rows (16 x 2048 x 8 x 64: 118 of 154 TFLOP/s), on short lines the loads in front of each
-// workgroup, which two waves per SIMD do not cover (256 ragged lines of 150 x 8 x 50: 131 us, 46 of them matrix time).  Packed documents
-// (8192 steps, 24 of them, 16 x 128 bf16): 72 + 5 us, most of it the latency of 1 to 16 tiles per workgroup.
-// 128 queries a workgroup where rows are long: keys are read from the L2 half as often; 64 on short lines (131 against 200 us for the lines above).
+// 161 us, 335 TFLOP/s.  fp32 the matrix units on long rows (16 x 2048 x 8 x 64: 118 of 154 TFLOP/s), on short lines the loads in front of each
+// workgroup, which two waves per SIMD do not cover (256 ragged lines of 150 x 8 x 50: 132 us, 46 of them matrix time).  Packed documents
+// (8192 steps, 24 of them, 16 x 128 bf16): 73 + 5 us, most of it the latency of 1 to 16 tiles per workgroup.
+// 128 queries a workgroup where rows are long: keys are read from the L2 half as often; 64 on short lines (131 against 200 us for the lines above when it was chosen).
 #include "attn_seq.h"
 
 namespace {
@@ -242,6 +242,7 @@ __global__ __launch_bounds__(NW * 64, EP * sizeof(T) > 256 ? 1 : 2) void attn_ti
     // in part can do that; they are searched while they go to LDS.
     auto search = [&](int t) { return docs || (t + 1) * BK > bmin; };
     constexpr bool ONE = NT % CPR == 0;                                   // a thread's chunks are all of the same channels
+    // (ANDed with a mask kept in registers: 131 -> 132.5 us on the lines above; chosen anew for every tile 137)
     const u32x4 all = {~0u, ~0u, ~0u, ~0u}, keep = own_chunk<T>(all, (int)threadIdx.x % CPR * CV, a.E);
     auto put = [&](int t, int buf, int turn) {
         bool hit = false;
