@@ -6,9 +6,9 @@
 // scores lie.  16-bit types: 32x32x16, V^T by transposing LDS reads (ds_read_b64_tr_b16) from row-major tiles.  fp32: the exact 32x32x2.
 // Key tiles pass through two LDS buffers, the next one's loads are in flight while a tile is computed; one barrier a tile.
 //
-// What bounds it: 16-bit heads of 64 channels the vector units (per score a multiply-add, an exponential, a maximum, a sum and half a conversion
-// against 16 matrix instructions per 64 x 32 scores; the cap adds an exponential and a reciprocal): 2 x 4000 x 16 x 64 fp16, capped, causal with a prefix:
-// 161 us, 335 TFLOP/s.  fp32 the matrix units on long rows (16 x 2048 x 8 x 64: 118 of 154 TFLOP/s), on short lines the loads in front of each
+// What bounds it: 16-bit heads of 64 channels the vector units (per score a multiply-add, an exponential, a maximum, a sum and two to three for the weight in two parts
+// against 24 matrix instructions per 64 x 32 scores; the cap adds an exponential and a reciprocal): 2 x 4000 x 16 x 64 fp16, capped, causal with a prefix:
+// 184 us, 293 TFLOP/s.  fp32 the matrix units on long rows (16 x 2048 x 8 x 64: 118 of 154 TFLOP/s), on short lines the loads in front of each
 // workgroup, which two waves per SIMD do not cover (256 ragged lines of 150 x 8 x 50: 132 us, 46 of them matrix time).  Packed documents
 // (8192 steps, 24 of them, 16 x 128 bf16): 73 + 5 us, most of it the latency of 1 to 16 tiles per workgroup.
 // 128 queries a workgroup where rows are long: keys are read from the L2 half as often; 64 on short lines (131 against 200 us for the lines above when it was chosen).
@@ -29,6 +29,23 @@ __device__ __forceinline__ f32x16 mfma16(f16_t, const s16x8& a, const s16x8& b, 
     return __builtin_amdgcn_mfma_f32_32x32x16_f16(__builtin_bit_cast(f16x8, a), __builtin_bit_cast(f16x8, b), c, 0, 0, 0);
 }
 __device__ __forceinline__ f32x16 mfma16(float, const s16x8&, const s16x8&, const f32x16& c) { return c; }
+
+// Two weights, each as the sum of two numbers of the type: the nearest one, and what is left of the weight.
+typedef float f32x2 __attribute__((ext_vector_type(2)));
+__device__ __forceinline__ void two_parts(f16_t, f32x2 w, unsigned& first, unsigned& rest) {
+    typedef _Float16 f16x2 __attribute__((ext_vector_type(2)));
+    first = __builtin_bit_cast(unsigned, __builtin_convertvector(w, f16x2));
+    f32x2 r;                                                       // w - first, the half of a word as operand: no conversion back
+    asm("v_fma_mix_f32 %0, -%1, 1.0, %2 op_sel_hi:[1,0,0]" : "=v"(r.x) : "v"(first), "v"(w.x));
+    asm("v_fma_mix_f32 %0, -%1, 1.0, %2 op_sel:[1,0,0] op_sel_hi:[1,0,0]" : "=v"(r.y) : "v"(first), "v"(w.y));
+    rest = __builtin_bit_cast(unsigned, __builtin_convertvector(r, f16x2));
+}
+__device__ __forceinline__ void two_parts(bf16_t, f32x2 w, unsigned& first, unsigned& rest) {
+    typedef __bf16 bf16x2 __attribute__((ext_vector_type(2)));
+    first = __builtin_bit_cast(unsigned, __builtin_convertvector(w, bf16x2));
+    const f32x2 r = {w.x - __builtin_bit_cast(float, first << 16), w.y - __builtin_bit_cast(float, first & 0xffff0000u)};
+    rest = __builtin_bit_cast(unsigned, __builtin_convertvector(r, bf16x2));
+}
 
 // A head is read in chunks of 16 bytes; where its E channels are no whole number of them, the last chunk is loaded so that it ENDS there: one load
 // without a condition whatever E is, and none past the row.  Its first channels are in the chunk before as well: values are kept so,
@@ -123,6 +140,8 @@ __global__ __launch_bounds__(NW * 64, EP * sizeof(T) > 256 ? 1 : 2) void attn_ti
     using G = Geo<T, EP, NW>;
     constexpr bool F32 = G::F32;
     constexpr int BK = G::BK, SB = G::SB, EB = G::EB, KLD = G::KLD, VLD = G::VLD, CV = G::CV, NT = NW * 64;
+    // fp16 weights are raised by 2^7, to 2^15 at most: their smallest step, 2^-24, is then 2^-31 of the row's largest weight
+    constexpr float LIFT = __is_same(T, f16_t) ? 7.f : 0.f;
     constexpr int NJ = !F32 && NW == 4 && EP <= 64 ? 2 : 1;               // blocks of 32 keys at once: more to overlap, where the registers allow it
     constexpr int CPT = (G::CHUNKS + NT - 1) / NT, CPR = EP / CV;         // chunks per thread and per row
     __shared__ __attribute__((aligned(16))) T Kbuf[2][BK * KLD];
@@ -240,7 +259,8 @@ __global__ __launch_bounds__(NW * 64, EP * sizeof(T) > 256 ? 1 : 2) void attn_ti
 
     // A value that is not finite must not reach the queries that may not see it: 0 x NaN is NaN.  Only tiles that some query of the workgroup sees
     // in part can do that; they are searched while they go to LDS.
-    auto search = [&](int t) { return docs || (t + 1) * BK > bmin; };
+    // 16-bit types search every tile: their weights are two numbers, whose products with an infinity may be of either sign, or none at all.
+    auto search = [&](int t) { return !F32 || docs || (t + 1) * BK > bmin; };
     constexpr bool ONE = NT % CPR == 0;                                   // a thread's chunks are all of the same channels
     // (ANDed with a mask kept in registers: 131 -> 132.5 us on the lines above; chosen anew for every tile 137)
     const u32x4 all = {~0u, ~0u, ~0u, ~0u}, keep = own_chunk<T>(all, (int)threadIdx.x % CPR * CV, a.E);
@@ -390,13 +410,16 @@ __global__ __launch_bounds__(NW * 64, EP * sizeof(T) > 256 ? 1 : 2) void attn_ti
 #pragma unroll
                         for (int i = 0; i < 16; ++i) o[eb][i] *= f;
                 }
-                const float ref = m == -INFINITY ? 0.f : m;
+                const float ref = m == -INFINITY ? 0.f : m - LIFT;
                 float sum[4] = {0.f, 0.f, 0.f, 0.f};
                 EACH(s[x][i] = __builtin_amdgcn_exp2f(__builtin_fmaf(s[x][i], scale, -ref)); sum[i % 4] += s[x][i]);
                 l += (sum[0] + sum[1]) + (sum[2] + sum[3]);
 
                 // O^T += V^T P^T
                 unsigned seen[NJ];                                        // of this half's keys, those with a weight
+                if (bad) {
+                    EACH(seen[x] = (i ? seen[x] : 0u) | (s[x][i] != 0.f ? 1u << (8 * (i / 4) + i % 4) : 0u));
+                }
                 if constexpr (F32) {
 #pragma unroll
                     for (int eb = 0; eb < EB; ++eb)
@@ -407,25 +430,36 @@ __global__ __launch_bounds__(NW * 64, EP * sizeof(T) > 256 ? 1 : 2) void attn_ti
                             for (int i = 0; i < 16; ++i)
                                 o[eb] = __builtin_amdgcn_mfma_f32_32x32x2f32(vb[(8 * (i / 4) + i % 4) * VLD], s[x][i], o[eb], 0, 0, 0);
                         }
-                    if (bad) {
-                        EACH(seen[x] = (i ? seen[x] : 0u) | (s[x][i] != 0.f ? 1u << (8 * (i / 4) + i % 4) : 0u));
-                    }
                 } else {
-                    s16x8 p[2 * NJ];                                      // weights in the values' type, half a step each; the sum l keeps them whole
-                    EACH(p[2 * x + i / 8][i % 8] = __builtin_bit_cast(short, from_f<T>(s[x][i])));
+                    // Weights as two numbers of the values' type, a matrix instruction for each: the first alone is half a step off (2^-8 bf16,
+                    // 2^-11 fp16), more than the one rounding at the end; with the rest 2^-16 and 2^-22.  The first alone: capped prefix
+                    // 162 us instead of 184, documents 83 instead of 90.
+                    u32x4 p[2 * NJ], rest[2 * NJ];
+#pragma unroll
+                    for (int x = 0; x < NJ; ++x)
+#pragma unroll
+                        for (int i = 0; i < 16; i += 2) {
+                            unsigned first, left_over;
+                            two_parts(T{}, (f32x2){s[x][i], s[x][i + 1]}, first, left_over);
+                            p[2 * x + i / 8][i % 8 / 2] = first;
+                            rest[2 * x + i / 8][i % 8 / 2] = left_over;
+                        }
                     // lane l gets, for channel l % 32, the four keys of its half: 16 lanes hold four rows of 16 channels, read transposed
                     const T* vb = &Vs[(32 * b0 + 4 * half + (col & 15) / 4) * VLD + 16 * (col >> 4) + 4 * (col & 3)];
 #pragma unroll
-                    for (int eb = 0; eb < EB; ++eb)
+                    for (int x = 0; x < 2 * NJ; ++x) {                    // both parts of all channels in turn: part by part 93 us (documents)
+                        typedef __attribute__((address_space(3))) s16x4 lds4;
+                        s16x8 keys[EB];
 #pragma unroll
-                        for (int x = 0; x < 2 * NJ; ++x) {
-                            typedef __attribute__((address_space(3))) s16x4 lds4;
+                        for (int eb = 0; eb < EB; ++eb) {
                             const s16x4 lo = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds4*)&vb[16 * x * VLD + eb * 32]);
                             const s16x4 hi = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds4*)&vb[(16 * x + 8) * VLD + eb * 32]);
-                            o[eb] = mfma16(T{}, __builtin_shufflevector(lo, hi, 0, 1, 2, 3, 4, 5, 6, 7), p[x], o[eb]);
+                            keys[eb] = __builtin_shufflevector(lo, hi, 0, 1, 2, 3, 4, 5, 6, 7);
                         }
-                    if (bad) {
-                        EACH(seen[x] = (i ? seen[x] : 0u) | ((p[2 * x + i / 8][i % 8] & 0x7fff) ? 1u << (8 * (i / 4) + i % 4) : 0u));
+#pragma unroll
+                        for (int eb = 0; eb < EB; ++eb) o[eb] = mfma16(T{}, keys[eb], __builtin_bit_cast(s16x8, p[x]), o[eb]);
+#pragma unroll
+                        for (int eb = 0; eb < EB; ++eb) o[eb] = mfma16(T{}, keys[eb], __builtin_bit_cast(s16x8, rest[x]), o[eb]);
                     }
                 }
                 if (bad)                                                  // what an odd value does, to those that see it

@@ -828,3 +828,55 @@ def test_refusals_of_constrain_logits():
         constrain_logits(big[:2], out=big[1:])
     with pytest.raises(ValueError):
         label_mask([[40]], 40)
+
+
+# ------------------------------------------------------------------------------------------- weights of 16-bit attention keep their digits
+def whole_weights_ref(q, k, v, *args, **kw):
+    """`attention_ref` without its allowance for weights in 16 bits.  They are taken as the sum of two 16-bit numbers: half a step of half a
+    step off, 2^-16 (bf16) or 2^-22 (fp16) of the weight, and fp16's absolute half step of 2^-25 where the row's largest weight is 2^7 or more:
+    2^-32 of it, for every key."""
+    want, bound = attention_ref(q.float(), k.float(), v.float(), *args, **kw)
+    if q.dtype != torch.float32:
+        part, _ = attention_ref(q.float(), k.float(), v.float().abs(), *args, **kw)
+        bound = bound + part * (2.0 ** -16 if q.dtype == torch.bfloat16 else 2.0 ** -22)
+    if q.dtype == torch.float16:
+        bound = bound + 2.0 ** -32 * k.shape[1] * v.float().abs().max().item()
+    return want, bound
+
+
+@pytest.mark.parametrize('dtype', TYPES)
+@pytest.mark.parametrize('n,t,h,hk,e,lens,causal,prefix,docs,slopes,cap', [
+    (2, 3, 2, 1, 16, True, True, 0, 0, False, 0.0), (3, 150, 4, 4, 50, True, False, 0, 0, True, 0.0), (1, 300, 4, 2, 64, False, True, 90, 0, False, 30.0),
+    (1, 300, 4, 1, 128, False, True, 0, 5, False, 0.0), (1, 140, 2, 2, 200, False, False, 0, 0, False, 0.0), (2, 130, 2, 1, 13, True, True, 0, 3, True, 5.0),
+    (1, 1030, 2, 1, 96, False, True, 0, 0, False, 0.0)])
+def test_attention_is_rounded_once(dtype, n, t, h, hk, e, lens, causal, prefix, docs, slopes, cap):
+    q, k, v = qkv(n, t, t, h, hk, e, dtype, seed=11)
+    ls = ragged(n, t) if lens else None
+    pf = [prefix] * n if prefix else None
+    ids = torch.sort(torch.randint(0, docs, (n, t), generator=torch.Generator().manual_seed(4)), 1)[0].int().to(DEV) if docs else None
+    sl = slopes_of(h) if slopes else None
+    got = attention(q, k, v, ls, causal=causal, prefix_lens=pf, documents=ids, slopes=sl, cap=cap)
+    check(got, *whole_weights_ref(q, k, v, ls, ls, causal, 'start', pf, ids, sl, cap))
+
+
+@pytest.mark.parametrize('dtype', TYPES)
+@pytest.mark.parametrize('n,t,h,hk,e,slopes,cap', [(3, 50, 8, 2, 50, True, 0.0), (2, 700, 8, 1, 64, False, 10.0), (1, 3001, 6, 2, 80, True, 0.0)])
+def test_attention_step_is_rounded_once(dtype, n, t, h, hk, e, slopes, cap):
+    q, k, v = qkv(n, 1, t, h, hk, e, dtype, seed=12)
+    ls = ragged(n, t)
+    sl = slopes_of(h) if slopes else None
+    want, bound = whole_weights_ref(q, k, v, None, ls, align='end', slopes=sl, cap=cap)
+    check(attention_step(q[:, 0], k, v, ls, slopes=sl, cap=cap), want[:, 0], bound[:, 0])
+
+
+@pytest.mark.parametrize('dtype', TYPES)
+@pytest.mark.parametrize('causal', [False, True])
+def test_attention_infinite_values_that_every_query_sees(dtype, causal):
+    """A weight whose lower part is zero or negative must not turn an infinity into no number."""
+    q, k, v = qkv(1, 200, 200, 2, 1, 64, dtype, seed=14)
+    want = attention(q, k, v, causal=causal)
+    v[0, 0, 0, 7], v[0, 1, 0, 9] = math.inf, -math.inf
+    got = attention(q, k, v, causal=causal)
+    assert (got[..., 7] == math.inf).all() and (got[:, 1:, :, 9] == -math.inf).all()
+    rest = [c for c in range(64) if c not in (7, 9)]
+    assert torch.equal(got[..., rest], want[..., rest])
