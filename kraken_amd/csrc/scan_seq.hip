@@ -159,7 +159,9 @@ __global__ __launch_bounds__(256) void scan_seq_kernel(krk_scan_args a, ScanCut 
     }
 }
 
-// the states in front of every chunk: one lane per (channel, state), the chunks in order
+// The states in front of every chunk: one lane per (channel, state), the chunks in order.  A chunk's factor 2^(A sum) alone may leave float32's range
+// where the states do not (1e-30 under exp(6) for 20 steps, or an infinite state under a decay), so it is applied in two: a mantissa in (1/2, 1] and
+// the exponent by v_ldexp, which cannot overflow or vanish unless the state itself does.
 __global__ __launch_bounds__(256) void scan_join_kernel(krk_scan_args a, ScanCut cut) {
     const long id = (long)blockIdx.x * 256 + threadIdx.x, ds = (long)a.D * a.S;
     if (id >= ds) return;
@@ -181,7 +183,8 @@ __global__ __launch_bounds__(256) void scan_join_kernel(krk_scan_args a, ScanCut
 #pragma unroll
             for (int c = 0; c < B; ++c)
                 if (c0 + c < cut.chunks - 1) {
-                    h = h == 0.f ? q[c] : __builtin_fmaf(__builtin_amdgcn_exp2f(e[c] * A), h, q[c]);   // growth over a chunk may be infinite
+                    const float x = fminf(fmaxf(e[c] * A, -2000.f), 2000.f), up = ceilf(x);   // no number: q is none either
+                    h = __builtin_amdgcn_ldexpf(h * __builtin_amdgcn_exp2f(x - up), (int)up) + q[c];
                     p[(c0 + c) * ds] = h;
                 }
         }

@@ -880,3 +880,28 @@ def test_attention_infinite_values_that_every_query_sees(dtype, causal):
     assert (got[..., 7] == math.inf).all() and (got[:, 1:, :, 9] == -math.inf).all()
     rest = [c for c in range(64) if c not in (7, 9)]
     assert torch.equal(got[..., rest], want[..., rest])
+
+
+# ---------------------------------------------------------------------------------------- the scan's range does not depend on how it is cut
+@pytest.mark.parametrize('n', [1, 800])
+def test_selective_scan_small_state_under_growth(n):
+    """exp(6) a step for 20 steps, exp(-6) for 20: the state goes from 1e-30 to 1e22 and back, a chunk's factor passes float32's range.  One row is
+    cut into chunks, 800 rows are not.  Each of the up to 200 exponents is off by 6 / ln 2 steps of 2^-24 and the sums of a chunk's by as much again:
+    2 x 9 a step on top of the reference's 6."""
+    t, d, s = 200, 64, 4
+    dt = (torch.where(torch.arange(t) % 40 < 20, 1.0, -1.0) * torch.linspace(0.9, 1.0, d)[:, None]).t()[None].to(DEV).contiguous()
+    x, bc = torch.zeros(1, t, d, device=DEV), torch.ones(1, t, 1, s, device=DEV)
+    A, st = torch.full((d, s), 6.0, device=DEV), torch.full((1, d, s), 1e-30, device=DEV)
+    want, bound, want_after, bound_after = scan_ref(x, dt, A, bc, bc, None, softplus=False, state=st)
+    y, after = selective_scan(*(v.expand(n, -1, -1) for v in (x, dt)), A, *(bc.expand(n, -1, -1, -1),) * 2, state=st.expand(n, -1, -1))
+    for i in (0, n - 1):
+        check(y[i:i + 1], want, bound * 4)
+        check(after[i:i + 1], want_after, bound_after * 4)
+
+
+@pytest.mark.parametrize('n', [1, 800])
+def test_selective_scan_infinite_state_under_decay(n):
+    """An infinite state stays infinite as step by step, although its factor over a chunk is zero in float32."""
+    x, bc = torch.zeros(n, 200, 64, device=DEV), torch.ones(n, 200, 4, device=DEV)
+    y, after = selective_scan(x, torch.ones_like(x), torch.full((64, 4), -7.0, device=DEV), bc, bc, state=torch.full((n, 64, 4), math.inf, device=DEV))
+    assert (y == math.inf).all() and (after == math.inf).all()
