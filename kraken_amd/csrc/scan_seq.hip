@@ -26,6 +26,10 @@ struct ScanCut {
     float* sums;           // [N][chunks - 1][D]: sums of the steps
 };
 
+// A rate of -inf (a state that forgets at once) as the lowest number: a step of width zero, as the kernels take for one behind the end, then leaves the
+// state as it is, where 0 times -inf would be no number.  Steps not computed instead, one by one at the end: lines 87 -> 97 us, long row 160 -> 167.
+__device__ __forceinline__ float finite_rate(float a) { return fabsf(a) == INFINITY ? __builtin_copysignf(__FLT_MAX__, a) : a; }
+
 // SL states of a lane, four at a time; zeros where there are none
 template <int SL> __device__ __forceinline__ void load_states(const float* p, int n, float (&v)[SL]) {
 #pragma unroll
@@ -48,7 +52,7 @@ __global__ __launch_bounds__(256) void scan_seq_kernel(krk_scan_args a, ScanCut 
     float A[SL];
     load_states(a.A + (long)d * a.S + s0, a.S - s0, A);
 #pragma unroll
-    for (int j = 0; j < SL; ++j) A[j] *= LOG2E;
+    for (int j = 0; j < SL; ++j) A[j] = finite_rate(A[j] * LOG2E);
     const float bias = a.dt_bias ? a.dt_bias[d] : 0.f, skip = a.skip ? a.skip[d] : 0.f;
     for (int n = blockIdx.z; n < a.N; n += gridDim.z) {
         const int len = __builtin_amdgcn_readfirstlane(seq_len(a.lens, n, a.T));
@@ -166,7 +170,7 @@ __global__ __launch_bounds__(256) void scan_join_kernel(krk_scan_args a, ScanCut
     const long id = (long)blockIdx.x * 256 + threadIdx.x, ds = (long)a.D * a.S;
     if (id >= ds) return;
     const long d = id / a.S;
-    const float A = a.A[id] * LOG2E;
+    const float A = finite_rate(a.A[id] * LOG2E);
     for (int n = blockIdx.y; n < a.N; n += gridDim.y) {
         float h = a.state ? a.state[n * a.state_n + id] : 0.f;
         float* p = cut.part + (long)n * (cut.chunks - 1) * ds + id;
@@ -213,7 +217,7 @@ __global__ __launch_bounds__(256) void scan_step_kernel(krk_scan_args a) {
     if (on) {
 #pragma unroll
         for (int j = 0; j < 4; ++j) {
-            h[j] = __builtin_fmaf(__builtin_amdgcn_exp2f(s * A[j] * LOG2E), h[j], s * x * b[j]);
+            h[j] = __builtin_fmaf(__builtin_amdgcn_exp2f(s * finite_rate(A[j]) * LOG2E), h[j], s * x * b[j]);
             y = __builtin_fmaf(c[j], h[j], y);
         }
     }

@@ -905,3 +905,27 @@ def test_selective_scan_infinite_state_under_decay(n):
     x, bc = torch.zeros(n, 200, 64, device=DEV), torch.ones(n, 200, 4, device=DEV)
     y, after = selective_scan(x, torch.ones_like(x), torch.full((64, 4), -7.0, device=DEV), bc, bc, state=torch.full((n, 64, 4), math.inf, device=DEV))
     assert (y == math.inf).all() and (after == math.inf).all()
+
+
+@pytest.mark.parametrize('t', [1, 3, 8, 13, 200])
+def test_selective_scan_state_that_forgets_at_once(t):
+    """A = -inf: exp(s A) is 0 in every step, the state is s x B of the last one, whatever number of steps is computed together."""
+    c, _ = scan_inputs(2, t, 40, 4, 1, torch.float32, False)
+    c['A'][:20] = -math.inf
+    lens = torch.tensor([t, (t + 1) // 2])
+    want, bound, want_after, bound_after = scan_ref(**c, lens=lens)
+    y, after = selective_scan(**c, dt_softplus=True, seq_lens=lens)
+    check(y, want, bound)
+    check(after, want_after, bound_after)
+
+
+def test_selective_scan_no_step_of_a_state_that_forgets_at_once():
+    """A step of width zero leaves such a state too, in whole lines (cut and not) as in single steps."""
+    for n, t in ((2, 13), (1, 200)):
+        x, bc = torch.zeros(n, t, 8, device=DEV), torch.ones(n, t, 4, device=DEV)
+        A, st = torch.full((8, 4), -math.inf, device=DEV), rand(n, 8, 4)
+        y, after = selective_scan(x, x, A, bc, bc, state=st)
+        assert torch.equal(after, st) and y.isfinite().all()
+        one = st.clone()
+        selective_scan_step(x[:, 0], x[:, 0], A, bc[:, 0], bc[:, 0], state=one)
+        assert torch.equal(one, st)
