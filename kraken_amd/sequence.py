@@ -10,13 +10,14 @@ place.  Tensors are float32, bfloat16 or float16 on a HIP device, all of one typ
 
 Work goes to the current stream of the tensors' device; nothing synchronises, so calls with lengths on the device may be captured into a
 graph.  Lengths given on the host are checked; on the device they are clamped.  There is no backward pass: the library does not train, and a
-tensor that asks for a gradient is refused.  There is no CPU implementation here: without a HIP device every call raises.
+tensor that asks for a gradient, or carries one in forward mode, is refused.  There is no CPU implementation here: without a HIP device every call raises.
 """
 import ctypes as C
 import math
 from typing import Optional, Sequence, Union
 
 import torch
+from torch.autograd import forward_ad
 
 from . import _lib
 
@@ -25,6 +26,18 @@ __all__ = ['causal_conv', 'causal_conv_step', 'selective_scan', 'selective_scan_
 Lens = Union[torch.Tensor, Sequence[int], None]
 
 _TYPES = {torch.float32: _lib.TYPE_F32, torch.bfloat16: _lib.TYPE_BF16, torch.float16: _lib.TYPE_F16}
+
+
+def _no_dual():
+    """Whether no forward mode is on, in which a tensor may carry a tangent without requiring a gradient."""
+    return getattr(forward_ad, '_current_level', 0) < 0
+
+
+def _no_gradient(t, name):
+    if t.requires_grad and torch.is_grad_enabled():
+        raise ValueError(f'{name} requires a gradient: there is no backward pass, call under torch.no_grad()')
+    if not _no_dual() and forward_ad.unpack_dual(t).tangent is not None:
+        raise ValueError(f'{name} carries a forward gradient: there is no forward mode either')
 
 
 def _first(x, name, dim):
@@ -36,8 +49,7 @@ def _first(x, name, dim):
         raise ValueError(f'{name} has to be float32, bfloat16 or float16, not {x.dtype}')
     if x.dim() != dim:
         raise ValueError(f'{name} has to have {dim} axes, got {tuple(x.shape)}')
-    if x.requires_grad and torch.is_grad_enabled():
-        raise ValueError(f'{name} requires a gradient: there is no backward pass, call under torch.no_grad()')
+    _no_gradient(x, name)
     return x if x.stride(-1) == 1 or x.shape[-1] == 1 else x.contiguous()
 
 
@@ -45,7 +57,7 @@ def _like(t, name, shape, first, dtype=None, inner=1):
     """A tensor that goes with `first`: shape, type (first's unless given), device; its last `inner` axes adjacent (else a copy)."""
     if dtype is None:
         dtype = first.dtype
-    if isinstance(t, torch.Tensor) and t.shape == shape and t.dtype is dtype and t.device == first.device and not t.requires_grad and t.is_contiguous():
+    if isinstance(t, torch.Tensor) and t.shape == shape and t.dtype is dtype and t.device == first.device and not t.requires_grad and _no_dual() and t.is_contiguous():
         return t                                    # what a step of a stream passes, in one condition: it is called for every label
     if not isinstance(t, torch.Tensor) or t.shape != shape:
         raise ValueError(f'{name} has to be a tensor of shape {tuple(shape)}, got {tuple(t.shape) if isinstance(t, torch.Tensor) else type(t)}')
@@ -53,8 +65,7 @@ def _like(t, name, shape, first, dtype=None, inner=1):
         raise ValueError(f'{name} has to be {dtype}, not {t.dtype}')
     if t.device != first.device:
         raise ValueError(f'{name} is on {t.device}, the call on {first.device}')
-    if t.requires_grad and torch.is_grad_enabled():
-        raise ValueError(f'{name} requires a gradient: there is no backward pass, call under torch.no_grad()')
+    _no_gradient(t, name)
     if t.is_contiguous():
         return t
     want = 1

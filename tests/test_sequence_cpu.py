@@ -188,3 +188,19 @@ def test_penalties_that_float32_does_not_hold():
         with pytest.raises(ValueError):
             constraints._penalty(value, 'penalty', 2, None, positive)
     assert constraints._penalty(1.5, 'penalty', 2, None, True) == (None, 1.5)
+
+
+def test_forward_mode_is_refused():
+    """A dual tensor has requires_grad False: its tangent would be lost in silence."""
+    from torch.autograd import forward_ad
+    x = torch.rand(2, 3, 8)
+    with forward_ad.dual_level():
+        for t in (x, x[:, :, ::2].contiguous(), torch.rand(8)):
+            dual = forward_ad.make_dual(t, torch.ones_like(t))
+            with pytest.raises(ValueError, match='gradient'):
+                sequence._like(dual, 't', t.shape, x)
+            with torch.no_grad(), pytest.raises(ValueError, match='gradient'):
+                sequence._like(dual, 't', t.shape, x)
+            assert sequence._like(t, 't', t.shape, x) is t
+            assert sequence._like(torch.zeros(2, dtype=torch.int32), 't', (2,), x, torch.int32).dtype == torch.int32
+    assert sequence._like(x, 't', x.shape, x) is x

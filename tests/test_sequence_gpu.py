@@ -929,3 +929,20 @@ def test_selective_scan_no_step_of_a_state_that_forgets_at_once():
         one = st.clone()
         selective_scan_step(x[:, 0], x[:, 0], A, bc[:, 0], bc[:, 0], state=one)
         assert torch.equal(one, st)
+
+
+def test_forward_mode_is_refused():
+    """A dual tensor has requires_grad False: its tangent would be lost in silence."""
+    import torch.autograd.forward_ad as fwd
+    x, w = rand(2, 9, 8), rand(8, 4)
+    q, k, v = qkv(2, 9, 9, 4, 2, 16, torch.float32)
+    with fwd.dual_level():
+        dual = lambda t: fwd.make_dual(t, torch.ones_like(t))  # noqa: E731
+        for bad in (lambda: causal_conv(dual(x), w), lambda: causal_conv(x, dual(w)), lambda: attention(q, dual(k), v), lambda: attention_step(dual(q[:, 0]), k, v, [9, 9]),
+                    lambda: constrain_logits(dual(x)), lambda: constrain_logits(x, bias=dual(rand(8))), lambda: causal_conv_step(x[:, 0], w, state=dual(rand(2, 3, 8)))):
+            with pytest.raises(ValueError, match='gradient'):
+                bad()
+        assert torch.equal(causal_conv(x, w)[0], causal_conv(x, w)[0])
+    c, _ = scan_inputs(2, 9, 12, 4, 1, torch.float32, False)
+    with fwd.dual_level(), pytest.raises(ValueError, match='gradient'):
+        selective_scan(**dict(c, A=fwd.make_dual(c['A'], c['A'])))
