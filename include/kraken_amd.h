@@ -372,7 +372,7 @@ int krk_selective_scan(const krk_scan_args* args, void* stream);
  *     s = scale q.k;  cap > 0: s = cap tanh(s / cap);  slopes: s -= slopes[h] |p_i - j|;  softmax over the keys j that are allowed.
  * p_i = i, or with align_end k_len - q_len + i (the last valid query stands at the last valid key).  Key j is allowed for query i if
  * j < k_len, and documents[n][i] == documents[n][j] (Tq == Tk only), and, with causal, j <= p_i or j < prefix[n].
- * cap: 0 or a normal number; scale: finite.  A query without an allowed key, and every query i >= q_len, gives zeros.  Keys and values at j >= k_len are never used, whatever
+ * cap: 0 or a normal number; scale: within 2^127.  A query without an allowed key, and every query i >= q_len, gives zeros.  Keys and values at j >= k_len are never used, whatever
  * they hold; inside k_len a value that is not finite reaches only the queries that may see it.
  * q, out (N, Tq, H, E), k, v (N, Tk, Hk, E): E adjacent.  1 <= E <= 256.  krk_attention_workspace as for the scan.
  */

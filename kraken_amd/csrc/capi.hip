@@ -2715,7 +2715,7 @@ static int attention_args_ok(const krk_attention_args* a) {
     if (a->documents && a->Tq != a->Tk) return fail(KRK_E_INVALID, "krk_attention: documents need as many queries as keys");
     if (!(a->cap >= 0.f)) return fail(KRK_E_INVALID, "krk_attention: cap must not be negative");
     if (a->cap > 0.f && !std::isnormal(a->cap)) return fail(KRK_E_INVALID, "krk_attention: cap must be 0 or a normal number");
-    if (!std::isfinite(a->scale)) return fail(KRK_E_INVALID, "krk_attention: scale must be finite");
+    if (!(std::fabs(a->scale) <= 0x1p127f)) return fail(KRK_E_INVALID, "krk_attention: scale must be within 2^127");   // times log2 e: finite
     return KRK_OK;
 }
 

@@ -327,7 +327,10 @@ def _scores(q, h, e, slopes, cap, scale):
         slopes = _like(slopes, 'slopes', (h,), q, torch.float32)
     if 0 < cap < 2.0 ** -126:
         raise ValueError(f'cap has to be 0 or a normal float32, got {cap}')
-    return slopes, _finite(cap, 'cap', 0), e ** -0.5 if scale is None else _finite(scale, 'scale', -math.inf)
+    scale = e ** -0.5 if scale is None else _finite(scale, 'scale', -math.inf)
+    if abs(scale) > 2.0 ** 127:                     # its product with log2 e, the exponentials' base, has to be finite too
+        raise ValueError(f'scale has to be within 2^127, got {scale}')
+    return slopes, _finite(cap, 'cap', 0), scale
 
 
 def attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, seq_lens: Lens = None, *, key_lens: Lens = None, causal: bool = False,

@@ -204,3 +204,13 @@ def test_forward_mode_is_refused():
             assert sequence._like(t, 't', t.shape, x) is t
             assert sequence._like(torch.zeros(2, dtype=torch.int32), 't', (2,), x, torch.int32).dtype == torch.int32
     assert sequence._like(x, 't', x.shape, x) is x
+
+
+def test_scales_whose_exponent_float32_does_not_hold():
+    """The kernels' exponentials have the base 2: 3e38 times log2 e is infinite, and a score of zero times it no number."""
+    for scale in (3e38, -3e38):
+        with pytest.raises(ValueError, match='scale'):
+            sequence._scores(None, 2, 4, None, 0.0, scale)
+        assert _lib.load().krk_attention_workspace(ctypes.byref(attention_args(scale=scale))) == _lib.KRK_E_INVALID
+    assert sequence._scores(None, 2, 4, None, 0.0, -2.0 ** 127)[2] == -2.0 ** 127
+    assert _lib.load().krk_attention_workspace(ctypes.byref(attention_args(scale=2.0 ** 127))) >= 0
