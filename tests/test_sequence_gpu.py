@@ -946,3 +946,74 @@ def test_forward_mode_is_refused():
     c, _ = scan_inputs(2, 9, 12, 4, 1, torch.float32, False)
     with fwd.dual_level(), pytest.raises(ValueError, match='gradient'):
         selective_scan(**dict(c, A=fwd.make_dual(c['A'], c['A'])))
+
+
+# ------------------------------------------------------------------------------------------------- long key axes, many rows, a plan's output
+@pytest.mark.parametrize('dtype', TYPES)
+@pytest.mark.parametrize('h,e', [(1, 64), (2, 40)])
+def test_attention_documents_over_a_split_axis(dtype, h, e):
+    """Few heads on a long axis: it is split, and the documents' id ranges lie behind the partial sums in the workspace."""
+    q, k, v = qkv(2, 1500, 1500, h, 1, e, dtype)
+    ids = torch.randint(0, 5, (2, 1500), generator=torch.Generator().manual_seed(2)).int()
+    ids[1] = ids[1].sort()[0]
+    ids, lens = ids.to(DEV), [1401, 1500]
+    got = attention(q, k, v, lens, causal=True, documents=ids)
+    check(got, *attention_ref(q, k, v, lens, lens, True, documents=ids))
+
+
+@pytest.mark.parametrize('dtype', TYPES)
+def test_attention_more_tiles_than_bits(dtype):
+    """Enough workgroups that nothing is split, and more key tiles than the 64 whose masks are looked at together."""
+    q, k, v = qkv(64, 33, 4300, 8, 1, 16, dtype)
+    got = attention(q, k, v, key_lens=[4300] * 63 + [4097])
+    pick = [0, 31, 63]
+    check(got[pick], *attention_ref(q[pick], k[pick], v[pick], None, [4300, 4300, 4097]))
+
+
+@pytest.mark.parametrize('dtype', TYPES)
+@pytest.mark.parametrize('shuffled', [False, True])
+def test_attention_documents_of_more_tiles_than_bits(dtype, shuffled):
+    t, pick = 4300, [0, 9]
+    q, k, v = qkv(1, t, t, 16, 1, 16, dtype)
+    ids = torch.randint(0, 3, (1, t), generator=torch.Generator().manual_seed(5)).int()
+    ids = (ids if shuffled else ids.sort()[0]).to(DEV)
+    got = attention(q, k, v, [4291], documents=ids)
+    check(got[:, :, pick], *attention_ref(q[:, :, pick], k, v, [4291], [4291], documents=ids))
+
+
+@pytest.mark.parametrize('dtype', TYPES)
+def test_selective_scan_many_rows(dtype):
+    """More rows than a grid holds along one axis, and more than one step: the loop over rows."""
+    n, pick = 65600, [0, 1, 65534, 65535, 65536, 65599]
+    c, k = scan_inputs(n, 2, 3, 2, 1, dtype, True)
+    lens = torch.full((n,), 2)
+    lens[65536] = 1
+    y, after = selective_scan(**c, **k, dt_softplus=True, seq_lens=lens)
+    few = {m: (v[pick] if v.dim() > 2 else v) for m, v in {**c, **k}.items()}
+    want, bound, want_after, bound_after = scan_ref(**few, lens=lens[pick])
+    check(y[pick], want, bound)
+    check(after[pick], want_after, bound_after)
+
+
+def test_a_plans_output_through_the_operators():
+    """What a network gives goes in as it is, a view of time-major rows, with the lengths that the network gives: the decoder's classes are those
+    allowed, and scores that nothing constrains decode as they did."""
+    from tests.helpers import build_model, synth_input
+    from kraken_amd.ctc_decoder import greedy_decoder
+    from kraken_amd.specs import BENCH_A, bench_codec
+    m = build_model(BENCH_A, codec=bench_codec(), seed=0).to(DEV)
+    scores, lens = m.nn(synth_input(3, 400).to(DEV), torch.tensor([400, 250, 96]))
+    rows = scores.squeeze(2).transpose(1, 2)                             # (N, C, 1, T) -> (N, T, C), no copy
+    assert rows.stride(-1) == 1
+    classes = rows.shape[-1]
+    free = constrain_logits(rows, mask=label_mask([None] * 3, classes))
+    assert torch.equal(free, rows)
+    assert greedy_decoder(free.transpose(1, 2), lens) == greedy_decoder(scores.squeeze(2), lens)
+    allowed = [list(range(1, 40)), list(range(100, 200)), [7]]
+    lines = greedy_decoder(constrain_logits(rows, mask=label_mask(allowed, classes)).transpose(1, 2), lens)
+    assert any(lines) and all(lab in labels for line, labels in zip(lines, allowed) for lab, *_ in line)
+    heads = lambda v: v.unflatten(-1, (8, -1))  # noqa: E731
+    u, _ = causal_conv(rows, rand(classes, 4, seed=1, scale=0.5), None, lens)
+    want, bound, _ = conv_ref(rows, rand(classes, 4, seed=1, scale=0.5), None, lens, None, False, False)
+    check(u, want, bound)
+    check(attention(heads(rows), heads(u), heads(u), lens, causal=True), *attention_ref(heads(rows), heads(u), heads(u), lens, lens, True))
