@@ -6,6 +6,7 @@ kraken/lib/ctc_decoder.py:35-72, which takes the scores as they are): a form fie
 label of a label model.  Like the decoder it has no CPU implementation: without a HIP device the call raises.
 """
 import ctypes as C
+import operator
 from typing import Iterable, Optional, Union
 
 import numpy as np
@@ -31,7 +32,10 @@ def label_mask(allowed: Iterable[Optional[Iterable[int]]], classes: int, *, blan
         if labels is None:
             bits[:classes] = 1
         else:
-            labels = np.asarray(list(labels), dtype=np.int64)
+            try:
+                labels = np.asarray([operator.index(label) for label in labels], dtype=np.int64)
+            except TypeError as e:
+                raise ValueError(f'labels have to be whole numbers: {e}') from None
             if labels.size and (labels.min() < 0 or labels.max() >= classes):
                 raise ValueError(f'labels outside [0, {classes})')
             bits[labels] = 1

@@ -214,3 +214,15 @@ def test_scales_whose_exponent_float32_does_not_hold():
         assert _lib.load().krk_attention_workspace(ctypes.byref(attention_args(scale=scale))) == _lib.KRK_E_INVALID
     assert sequence._scores(None, 2, 4, None, 0.0, -2.0 ** 127)[2] == -2.0 ** 127
     assert _lib.load().krk_attention_workspace(ctypes.byref(attention_args(scale=2.0 ** 127))) >= 0
+
+
+def test_label_masks_of_what_is_no_label():
+    """1.7 is not label 1; whole numbers of any kind are labels."""
+    for bad in ([1.7], ['3'], [None]):
+        with pytest.raises(ValueError, match='whole numbers'):
+            constraints.label_mask([bad], 40, device='cpu')
+    want = constraints.label_mask([[1, 5]], 40, device='cpu')
+    for labels in (np.array([1, 5], dtype=np.int16), torch.tensor([1, 5]), {1, 5}, (5, 1), range(1, 6, 4), iter([1, 5])):
+        assert torch.equal(constraints.label_mask([labels], 40, device='cpu'), want)
+    with pytest.raises(ValueError, match='whole numbers'):
+        constraints.label_mask([torch.tensor([1.0])], 40, device='cpu')
