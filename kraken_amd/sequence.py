@@ -28,15 +28,10 @@ Lens = Union[torch.Tensor, Sequence[int], None]
 _TYPES = {torch.float32: _lib.TYPE_F32, torch.bfloat16: _lib.TYPE_BF16, torch.float16: _lib.TYPE_F16}
 
 
-def _no_dual():
-    """Whether no forward mode is on, in which a tensor may carry a tangent without requiring a gradient."""
-    return getattr(forward_ad, '_current_level', 0) < 0
-
-
 def _no_gradient(t, name):
     if t.requires_grad and torch.is_grad_enabled():
         raise ValueError(f'{name} requires a gradient: there is no backward pass, call under torch.no_grad()')
-    if not _no_dual() and forward_ad.unpack_dual(t).tangent is not None:
+    if forward_ad._current_level >= 0 and forward_ad.unpack_dual(t).tangent is not None:      # a dual tensor requires none itself
         raise ValueError(f'{name} carries a forward gradient: there is no forward mode either')
 
 
@@ -57,7 +52,8 @@ def _like(t, name, shape, first, dtype=None, inner=1):
     """A tensor that goes with `first`: shape, type (first's unless given), device; its last `inner` axes adjacent (else a copy)."""
     if dtype is None:
         dtype = first.dtype
-    if isinstance(t, torch.Tensor) and t.shape == shape and t.dtype is dtype and t.device == first.device and not t.requires_grad and _no_dual() and t.is_contiguous():
+    if (isinstance(t, torch.Tensor) and t.shape == shape and t.dtype is dtype and t.device == first.device and not t.requires_grad
+            and forward_ad._current_level < 0 and t.is_contiguous()):
         return t                                    # what a step of a stream passes, in one condition: it is called for every label
     if not isinstance(t, torch.Tensor) or t.shape != shape:
         raise ValueError(f'{name} has to be a tensor of shape {tuple(shape)}, got {tuple(t.shape) if isinstance(t, torch.Tensor) else type(t)}')
