@@ -325,7 +325,8 @@ int krk_upsample_sigmoid(const float* x_dev, int C, int h, int w, int H, int W, 
  * caller's, in ELEMENTS.  Ragged batches as everywhere here: only the first lens[n] steps of row n are valid (a DEVICE array, values
  * are clamped to [0, T]; NULL: all T), steps behind them are neither read nor left undefined: outputs there are zero.
  * Everything is enqueued on `stream`; nothing synchronises, allocates or keeps anything between calls, so the calls may be captured
- * into a graph.  Sums, softmax statistics and states are fp32; 16-bit results are rounded once, at the end.  Buffers that a call
+ * into a graph.  Sums, softmax statistics and states are fp32; 16-bit results are rounded once, at the end (softmax weights meet 16-bit values as
+ * two 16-bit numbers each, 2^-16 of a weight off or less).  How many rows a call has may decide how a long axis is cut, and with it last bits.  Buffers that a call
  * writes must not overlap anything else it is given, except where said.
  */
 #define KRK_TYPE_F32  0
@@ -373,7 +374,8 @@ int krk_selective_scan(const krk_scan_args* args, void* stream);
  * p_i = i, or with align_end k_len - q_len + i (the last valid query stands at the last valid key).  Key j is allowed for query i if
  * j < k_len, and documents[n][i] == documents[n][j] (Tq == Tk only), and, with causal, j <= p_i or j < prefix[n].
  * cap: 0 or a normal number; scale: within 2^127.  A query without an allowed key, and every query i >= q_len, gives zeros.  Keys and values at j >= k_len are never used, whatever
- * they hold; inside k_len a value that is not finite reaches only the queries that may see it.
+ * they hold; inside k_len a value that is not finite reaches only the queries that may see it.  The sums are formed of weights up to 2^8 (fp16: 2^15)
+ * and divided by theirs at the end: finite values of a size near float32's end (2^100 and more) may pass it.
  * q, out (N, Tq, H, E), k, v (N, Tk, Hk, E): E adjacent.  1 <= E <= 256.  krk_attention_workspace as for the scan.
  */
 typedef struct krk_attention_args {

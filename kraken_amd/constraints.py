@@ -3,7 +3,9 @@ Constraint of a network's scores in front of a decoder: the labels a line may ho
 
 ``constrain_logits`` stands between a network's scores and :func:`kraken_amd.ctc_decoder.greedy_decoder` (reference
 kraken/lib/ctc_decoder.py:35-72, which takes the scores as they are): a form field that holds digits only, a page in one script, or the next
-label of a label model.  Like the decoder it has no CPU implementation: without a HIP device the call raises.
+label of a label model.  It is for a loop of one's own over a network's ``nn(x)``; ``rpred`` and ``predict`` decode on the
+device and hand a custom decoder softmax values on the host, not scores.  Like the decoder it has no CPU implementation: without a HIP device
+the call raises.
 """
 import ctypes as C
 import operator

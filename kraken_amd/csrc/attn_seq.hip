@@ -287,8 +287,10 @@ int by_rows(const krk_attention_args& a, hipStream_t s) {
     }
 }
 
-// One or two query positions read the keys as often as they are rows; more of them go to the tile kernel, which reads them once per block.  Heads of
-// less than 16 bytes stay here: the tile kernel's loads are 16 bytes within a row.
+// One or two query positions read the keys as often as they are rows; more of them go to the tile kernel, which reads them once per block and query head.
+// Rows here and tiles, us: 16 caches of 8192, 32 heads on 8 x 128 bf16, two queries 160 / 389, three 212 / 390, six 378 / 389, eight 494 / 391;
+// 16 x 2048, 16 heads of 64 fp16 with keys of their own, two 32 / 44, four 42 / 45, six 56 / 45; 64 lines of 150, 8 x 50 fp32, two 14 / 21, three 22 / 22,
+// four 24 / 22.  Heads of less than 16 bytes stay here: the tile kernel's loads are 16 bytes within a row.
 bool by_tiles(const krk_attention_args& a) { return a.Tq > 2 && a.E * (a.type == KRK_TYPE_F32 ? 4 : 2) >= 16; }
 
 long part_bytes(const krk_attention_args& a, int splits) {

@@ -10,8 +10,8 @@
 // against 24 matrix instructions per 64 x 32 scores; the cap adds an exponential and a reciprocal): 2 x 4000 x 16 x 64 fp16, capped, causal with a prefix:
 // 184 us, 293 TFLOP/s.  fp32 the matrix units on long rows (16 x 2048 x 8 x 64: 118 of 154 TFLOP/s), on short lines the loads in front of each
 // workgroup, which two waves per SIMD do not cover (256 ragged lines of 150 x 8 x 50: 132 us, 46 of them matrix time).  Packed documents
-// (8192 steps, 24 of them, 16 x 128 bf16): 73 + 5 us, most of it the latency of 1 to 16 tiles per workgroup.
-// 128 queries a workgroup where rows are long: keys are read from the L2 half as often; 64 on short lines (131 against 200 us for the lines above when it was chosen).
+// (8192 steps, 24 of them, 16 x 128 bf16): 78 + 5 us, most of it the latency of 1 to 16 tiles per workgroup.  Both units are far from full there: the
+// vector units issue in 43 % of the CUs' busy cycles and the matrix units run in 25 % (capped prefix 63 and 21 %), at 1.6 to 1.9 waves per SIMD.
 #include "attn_seq.h"
 
 namespace {
@@ -561,12 +561,14 @@ int by_width(const krk_attention_args& a, const AttnTiles& g, void* scratch, hip
 
 AttnTiles krk_attn_tiles(const krk_attention_args& a) {
     AttnTiles g;
-    // a block of 128 queries reads the keys half as often, but leaves more of it empty on short lines; wide heads have no registers for 64
+    // A block of 128 queries reads the keys half as often, but leaves more of it empty on short lines: 8 heads of 50 fp32, 65536 steps in all, rows of
+    // 192 284 us with 64 and 353 with 128, 256 363 / 333, 300 470 / 518, 384 516 / 472, 1024 1268 / 1177.  Wide heads have no registers for two waves.
     const bool f32 = a.type == KRK_TYPE_F32;
     g.rows = a.Tq > 256 || a.E > (f32 ? 64 : 128) ? 128 : 64;
     g.keys = f32 || g.rows == 64 ? 32 : 64;
     const long blocks = (long)a.N * a.H * ((a.Tq + g.rows - 1) / g.rows), tiles = (a.Tk + g.keys - 1) / g.keys;
-    // few workgroups and a long axis: split it, eight tiles at least to each
+    // Few workgroups and a long axis: split it, eight tiles at least to each (64 queries of 8 heads x 64 fp32 on 2048 keys: 31 us, with four tiles at least 21,
+    // with sixteen 52; 512 of 4 x 128 fp16 on 16384: 49, 48, 53).
     g.splits = (int)max(1L, min(min((512 + blocks - 1) / max(blocks, 1L), tiles / 8), 64L));
     g.range_bytes = a.documents ? (long)a.N * tiles * 8 : 0;
     return g;

@@ -9,7 +9,7 @@
 
 namespace {
 
-constexpr int CH = 4096;      // classes of a workgroup: 16 KB of counters, ten workgroups per CU
+constexpr int CH = 4096;      // classes of a workgroup: 16 KB of counters, eight workgroups (all that the waves allow) in 128 of a CU's 160 KB
 
 // MANY: more lines than a grid has; a loop over lines in every call costs a quarter of its speed (12 -> 15.7 us)
 template <class T, class I, bool MANY>
@@ -75,7 +75,7 @@ int launch(const krk_constrain_args& a, hipStream_t s) {
     const int chunks = (a.C + CH - 1) / CH, groups = (min(a.C, CH) + V - 1) / V;
     int bits = 0;
     while (bits < 8 && (1 << bits) < groups) ++bits;
-    // steps of a workgroup: enough that counting the history is paid for, as many workgroups as eight per CU
+    // steps of a workgroup: enough that counting the history is paid for, up to sixteen workgroups per CU
     int rows = 256 >> bits;
     while ((long)a.N * chunks * ((a.T + rows - 1) / rows) > 4096 && rows < a.T) rows *= 2;
     const int parts = (a.T + rows - 1) / rows;

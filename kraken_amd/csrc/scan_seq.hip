@@ -7,12 +7,12 @@
 // registers for a whole row; lanes lie along the channels, so every access of a step is contiguous.  B and C, the same for all channels of a
 // group, go through LDS as fp32, U steps at a time; the next U steps' inputs are in flight while U steps are computed.
 // Of a step's 125 vector instructions 80 are the states' (16 of them exponentials, at half rate), so 580 cycles a wave: 256 ragged lines of
-// 150 x 400 x 16 fp32 would take 39 us on evenly filled SIMDs and take 85 (1600 waves of different lengths on 1024 SIMDs); blocks of 64 or 128
-// lanes instead of 256 make no difference.
+// 150 x 400 x 16 fp32 would take 39 us on evenly filled SIMDs and take 85: eight waves a row, 2048 of different lengths on 1024 SIMDs, and as a block
+// holds channels of one row only, the last of the eight has none and computes all the same; blocks of 64 or 128 lanes instead of 256 make no difference.
 //
 // Few rows do not fill the chip with channels alone: then the time axis is cut into chunks.  One pass gives every chunk's end state from a
 // zero start and the sum of its steps -- the decay over a chunk is exp(A sum) --, a second joins the chunks in order, and the main pass starts every
-// chunk from its true state (1 x 8191 x 2048 x 16 bf16: 67 + 8 + 90 us; in one pass 26 ms).  That costs four fifths of the work again, so it is done only where a quarter of the SIMDs would idle.
+// chunk from its true state (1 x 8191 x 2048 x 16 bf16: 68 + 9 + 90 us; in one pass 26 ms).  That costs four fifths of the work again, so it is done only where a quarter of the SIMDs would idle.
 #include "seq.h"
 
 namespace {
@@ -234,7 +234,9 @@ __global__ __launch_bounds__(256) void scan_step_kernel(krk_scan_args a) {
 int lanes_of(int S) { return S <= 16 ? 1 : S <= 64 ? 4 : 16; }
 
 // Chunks of the time axis: none while the channels give one wave per SIMD or the rows are short; else enough for two waves each, 16 steps at least
-// (1 x 1000 x 500 x 16: 35 us against 43 with 32 and 63 with 64 steps at least).
+// (1 x 1000 x 500 x 16: 35 us against 43 with 32 and 63 with 64 steps at least).  Cut and whole, lines of 150 x 400 fp32: 32 of them 49 / 66 us, 64 58 / 67,
+// 96 85 / 67, 128 93 / 67; lines of 150 x 64: 64 of them 41 / 65, 128 64 / 65, 256 88 / 66; rows of 1000 x 512: 64 of them 289 / 413, 96 428 / 428.
+// The rule counts channels, not the waves launched, which on narrow rows are up to four times as many.
 void cut_time(const krk_scan_args& a, ScanCut& c) {
     const long waves = (long)a.N * a.D * lanes_of(a.S) / 64 + 1;
     long chunks = waves > 768 ? 1 : min((long)a.T / 16, 2048 / waves);

@@ -3,7 +3,8 @@ Operators on sequence rows: a short causal convolution, a selective state space 
 line's time axis, next to the LSTM layers of :mod:`kraken_amd.vgsl` (the reference's only one, kraken/lib/vgsl/layers.py:462-547).
 
 They take and give what a network's sequence layers do here: time-major rows ``(N, T, channels)``, right-padded, with ``seq_lens`` valid
-steps per line.  Padding is never read, whatever it holds, and is zero in the result, so a line does not depend on its batch.  A recurrence
+steps per line.  Padding is never used, whatever it holds, and is zero in the result, so a line does not depend on what else is in its
+batch; on how MANY lines there are the last bits of a scan or of attention may depend, since few lines are cut along their axis.  A recurrence
 runs in either direction and carries its state from call to call; the ``_step`` forms take one step per line and update the state in
 place.  Tensors are float32, bfloat16 or float16 on a HIP device, all of one type; sums, softmax statistics and states are float32, and a
 16-bit result is rounded once.  Channels that are not adjacent in memory are laid out first (a copy); every other stride is taken as it is.
