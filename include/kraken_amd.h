@@ -352,6 +352,8 @@ int krk_causal_conv(const krk_conv_args* args, void* stream);
  * Selective state space scan, per channel d of group g = d / (D / G) with S states:
  *     s_i = dt_i + dt_bias (softplus of it with `softplus`),  h_i = exp(s_i A) h_{i-1} + s_i x_i B_i,  y_i = C_i . h_i + skip x_i,
  *     times z_i sigmoid(z_i) when z is given.
+ * A step width or input that is not finite leaves its channel, from that step on, without finite results: infinite or no number.
+ * Rates may be -inf: such a state holds the last step's input alone, and a width of zero leaves it as it is.
  * Processing order, lens and padding as above.  A (D, S), skip (D), dt_bias (D) and the states (N, D, S) are fp32; skip, dt_bias, z,
  * state (zero) and state_out may be NULL.  B, C (N, T, G, S): (G, S) adjacent.  With T == 1 state_out may be state itself.
  * 1 <= S <= 256.  krk_selective_scan_workspace: bytes of device scratch that the call needs for these sizes (0: none; negative: error).

@@ -55,8 +55,14 @@ __device__ __forceinline__ float seq_silu(float p) { return p * __builtin_amdgcn
 
 // softplus(v) = max(v, 0) + log1p(e), e = exp(-|v|) in (0, 1].  log1p(e) = 2 atanh(r), r = e / (2 + e) <= 1/3, by its odd series up to r^15
 // (the rest is below 2^-27 of it): one exp, one rcp, and full relative accuracy where the result is tiny, which log(1 + e) does not have.
+// The exponent's product with log2 e would be off by |v| 2^-24, which a step width passes on whole; what its rounding and the constant's lose
+// goes into e as a factor 1 + loss ln 2.
 __device__ __forceinline__ float seq_softplus(float v) {
-    const float e = __expf(-fabsf(v));
+    constexpr float L = 1.4426950408889634f, REST = (float)(1.4426950408889634 - (double)L), LN2 = 0.6931471805599453f;
+    const float a = fabsf(v) > 200.f ? 200.f : fabsf(v), t = a * L;    // beyond 200: e is zero, and an infinite a would have no rest
+    const float loss = __builtin_fmaf(a, REST, __builtin_fmaf(a, L, -t));
+    float e = __builtin_amdgcn_exp2f(-t);
+    e = __builtin_fmaf(e, loss * -LN2, e);
     const float r = e * __builtin_amdgcn_rcpf(2.f + e), q = r * r;
     float p = 2.f / 15.f;
     p = __builtin_fmaf(p, q, 2.f / 13.f);

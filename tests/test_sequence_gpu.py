@@ -1017,3 +1017,24 @@ def test_a_plans_output_through_the_operators():
     want, bound, _ = conv_ref(rows, rand(classes, 4, seed=1, scale=0.5), None, lens, None, False, False)
     check(u, want, bound)
     check(attention(heads(rows), heads(u), heads(u), lens, causal=True), *attention_ref(heads(rows), heads(u), heads(u), lens, lens, True))
+
+
+def test_selective_scan_steps_within_ten_roundings():
+    """softplus over its whole range, y = s x of one state's first step: exp2 2 steps of 2^-24, its correction 1, 2 + e 1/3, the reciprocal 2, their
+    product 1, the series 1.3 and the last sum 1."""
+    v = torch.cat([torch.linspace(-80, 80, 16001), torch.linspace(-4, 4, 8001), torch.tensor([0.0, -300.0, 300.0, math.inf, -math.inf])]).to(DEV)
+    one, d = torch.ones(1, 1, len(v), device=DEV), len(v)
+    unit = torch.ones(1, 1, 1, device=DEV)
+    y, _ = selective_scan(one, v.view(1, 1, -1), -torch.ones(d, 1, device=DEV), unit, unit, dt_softplus=True)
+    y2 = selective_scan(one.expand(1, 20, d), v.expand(1, 20, d), torch.full((d, 1), -math.inf, device=DEV), unit.expand(1, 20, 1), unit.expand(1, 20, 1),
+                        dt_softplus=True)[0][:, -1:]
+    want = torch.nn.functional.softplus(v.double(), threshold=1000)
+    # an infinite width leaves its channel without a finite result: infinity, or none at all (times the zeros that fill a lane's set of states up)
+    assert not y[0, 0][want == math.inf].isfinite().any()
+    for got in (y, y2):
+        got = got[0, 0].double()
+        low = want < 1e-36                                                                        # results without full precision
+        assert ((got - want).abs()[~low & want.isfinite()] <= 10 * U * want[~low & want.isfinite()]).all()
+        assert (got[low].abs() <= 2e-36).all()
+    bad = torch.full((1, 1, 4), math.nan, device=DEV)
+    assert selective_scan(torch.ones_like(bad), bad, -torch.ones(4, 1, device=DEV), unit, unit, dt_softplus=True)[0].isnan().all()
