@@ -6,13 +6,13 @@
 // units bound it, not memory.  A lane owns a channel (LP lanes share one with more than SL states) and keeps its states and rates in
 // registers for a whole row; lanes lie along the channels, so every access of a step is contiguous.  B and C, the same for all channels of a
 // group, go through LDS as fp32, U steps at a time; the next U steps' inputs are in flight while U steps are computed.
-// Of a step's 125 vector instructions 80 are the states' (16 of them exponentials, at half rate), so 580 cycles a wave: 256 ragged lines of
-// 150 x 400 x 16 fp32 would take 39 us on evenly filled SIMDs and take 85: eight waves a row, 2048 of different lengths on 1024 SIMDs, and as a block
+// Of a step's 132 vector instructions 80 are the states' (16 of them exponentials, at half rate), so 590 cycles a wave: 256 ragged lines of
+// 150 x 400 x 16 fp32 would take 40 us on evenly filled SIMDs and take 87: eight waves a row, 2048 of different lengths on 1024 SIMDs, and as a block
 // holds channels of one row only, the last of the eight has none and computes all the same; blocks of 64 or 128 lanes instead of 256 make no difference.
 //
 // Few rows do not fill the chip with channels alone: then the time axis is cut into chunks.  One pass gives every chunk's end state from a
 // zero start and the sum of its steps -- the decay over a chunk is exp(A sum) --, a second joins the chunks in order, and the main pass starts every
-// chunk from its true state (1 x 8191 x 2048 x 16 bf16: 68 + 9 + 90 us; in one pass 26 ms).  That costs four fifths of the work again, so it is done only where a quarter of the SIMDs would idle.
+// chunk from its true state (1 x 8191 x 2048 x 16 bf16: 71 + 9 + 95 us; in one pass 3.6 ms).  That costs four fifths of the work again, so it is done only where a quarter of the SIMDs would idle.
 #include "seq.h"
 
 namespace {
