@@ -35,7 +35,9 @@ typedef float f32x2 __attribute__((ext_vector_type(2)));
 __device__ __forceinline__ void two_parts(f16_t, f32x2 w, unsigned& first, unsigned& rest) {
     typedef _Float16 f16x2 __attribute__((ext_vector_type(2)));
     first = __builtin_bit_cast(unsigned, __builtin_convertvector(w, f16x2));
-    f32x2 r;                                                       // w - first, the half of a word as operand: no conversion back
+    // w - first, with half a word as operand: no conversion back.  An exponential's result must not be read by the very next instruction, which the
+    // compiler does not see to for assembly: the conversion above stands in between.
+    f32x2 r;
     asm("v_fma_mix_f32 %0, -%1, 1.0, %2 op_sel_hi:[1,0,0]" : "=v"(r.x) : "v"(first), "v"(w.x));
     asm("v_fma_mix_f32 %0, -%1, 1.0, %2 op_sel:[1,0,0] op_sel_hi:[1,0,0]" : "=v"(r.y) : "v"(first), "v"(w.y));
     rest = __builtin_bit_cast(unsigned, __builtin_convertvector(r, f16x2));
